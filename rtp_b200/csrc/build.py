@@ -11,7 +11,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(os.path.dirname(HERE), "lib")
 LIB_PATH = os.path.join(LIB_DIR, "librtp_b200.so")
-SOURCES = ["gemm.cu", "gemm_local.cu", "kernels.cu", "attn_tc.cu", "flash_attn.cu", "ring_shift.cu", "gate_rope.cu", "im2col.cu", "noalloc.cu"]
+SOURCES = ["gemm.cu", "gemm_local.cu", "kernels.cu", "attn_tc.cu", "flash_attn.cu", "ring_shift.cu", "gate_rope.cu", "rotary.cu", "im2col.cu", "noalloc.cu"]
 # sources with many variants of a kernel, compiled in parts side by side: the macro that names a part, their number
 PARTS = {"flash_attn.cu": ("RTP_FLASH_PART", 4)}
 NVCC_FLAGS = [

@@ -78,6 +78,23 @@ int rtp_top2_gate_bwd(const float* gates, const int* idx, const unsigned char* v
                       const float* d_gate_w, const float* d_l_aux, float* dlogits, int S, int E, void* stream);
 int rtp_rope(const void* x, void* y, const float* cosv, const float* sinv, long long T, int H, int hd, int S, int inner,
              int backward, void* stream);
+// Rotary positions of q and k (rotary.cu): views [B, S, heads, hd] with unit stride inside a head (strides in elements) in, contiguous
+// [B, S, heads, hd] out; k_heads = 0: q alone.  Pair i of the first `rot` elements turns by positions[b, s] * freqs[i] radians.
+typedef struct {
+  const void *q, *k;
+  void *qo, *ko;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh;
+  const void* positions;               // int64 (pos64 = 1) or int32 at b * pos_sb + s * pos_ss
+  long long pos_sb, pos_ss;
+  const double* freqs;                 // [rot / 2]
+  float magnitude;                     // factor on the rotated part
+  int pos64, B, S, q_heads, k_heads, hd, rot;
+  int half_layout;                     // 1: pairs (i, i + rot / 2), 0: (2 i, 2 i + 1)
+  int dtype;                           // 0 bf16, 1 fp16, 2 fp32
+  int backward;                        // 1: the transposed map
+} RtpRotary;
+int rtp_rotary(const RtpRotary* args, void* stream);
+const char* rtp_rotary_last_error(void);
 // Convolution as GEMM: patch matrix of an NCHW bf16 input and its adjoint (im2col.cu).
 const char* rtp_im2col_last_error(void);
 int rtp_im2col(const void* x, void* cols, int B, int C, int H, int W, int KH, int KW, int sh, int sw, int ph, int pw,

@@ -297,6 +297,19 @@ def rope_attention_packed(qkv, cos, sin, heads, nshard=1):
     return None
 
 
+def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
+    """Rotary positions: turns the pairs of the first ``rotary_dim`` elements of every head of ``q`` [B, S, H, hd] and ``k``
+    [B, S, Hk, hd] (None: q alone; any strides) by ``positions * freqs`` radians and returns new (q, k).
+
+    ``positions``: int64 / int32 [S] or [B, S], any values.  ``freqs``: float64 [rotary_dim / 2], see
+    ``ops.rotary.rotary_frequencies``.  ``layout``: pairs ``(x[i], x[i + rotary_dim / 2])`` for ``"half"``, ``(x[2i], x[2i + 1])`` for
+    ``"interleaved"``.  ``magnitude``: factor on the rotated part (``ops.rotary.rotary_magnitude``)."""
+    from . import rotary as R
+    if R.kernel_takes(q) and get_backend() != "functional":
+        return R.rotary(q, k, positions, freqs, layout, magnitude)
+    return R.rotary_plain(q, k, positions, freqs, layout, magnitude)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # LM head + cross-entropy without the [tokens, vocab] logits
 # ---------------------------------------------------------------------------------------------------------------------
