@@ -80,6 +80,9 @@ struct MaskArgs {
   uint32_t thresh; float drop_scale;
   unsigned long long seed, offset;
   const unsigned long long* step_ptr;
+  // window (MSK 3): query i stands at position i + ahead and sees keys j <= i + ahead that are among the last `window` of those or the
+  // first `sinks` of all
+  int window, sinks, ahead;
 };
 
 struct alignas(64) FlashParams {
@@ -91,6 +94,10 @@ struct alignas(64) FlashParams {
   int B, H;
   int group;                           // (batch, head) pairs whose CTAs run side by side (see head_group)
   int split;                           // forward: one row tile a CTA, its key blocks dealt to the two warpgroups
+  // window: query heads that share a key head; key blocks that hold a sink; the first of the others that a query sees; pieces that the
+  // queries of a block of sinks fall into, and where those leave their sums (null: one piece)
+  int qpk, sink_blocks, first_block, pieces;
+  float* part;
   MaskArgs m;
   unsigned long long* status;
   unsigned long long timeout_ns;
@@ -150,9 +157,12 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   }
 }
 
+// the bits below bit n (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 // x[i] = log2-domain score of (row, col0 + i): scale, additive mask, key padding, causal and sequence bounds.
 // Masked entries become -inf.  `plain` = nothing but the scale applies to this block.  MSK: 0 no masks, 1 key padding only,
-// 2 an additive mask (with or without key padding); `dead`: bit i set = key col0 + i is padding (dead_keys).
+// 2 an additive mask (with or without key padding), 3 window and sinks; `dead`: bit i set = key col0 + i is padding (dead_keys).
 template <int NC, int MSK>
 __device__ __forceinline__ void score_chunk(float* x, int row, int col0, uint32_t dead, const MaskArgs& m, bool plain) {
   static_assert(NC == 32, "one word of bits");
@@ -193,7 +203,13 @@ __device__ __forceinline__ void score_chunk(float* x, int row, int col0, uint32_
   }
   // bit i: key col0 + i has no weight
   uint32_t off = MSK ? dead : 0u;
+  if constexpr (MSK == 3) {
+    const int pos = row + m.ahead;
+    off |= below(pos + 1 - col0) ^ 0xffffffffu;                                    // after the query
+    off |= below(pos + 1 - m.window - col0) & ~below(m.sinks - col0);              // before its window, no sink
+  } else {
   if (m.causal && col0 + NC - 1 > row) off |= row < col0 ? 0xffffffffu : 0xffffffffu << (row + 1 - col0);
+  }
   if (col0 + NC > m.Sk) off |= col0 >= m.Sk ? 0xffffffffu : 0xffffffffu << (m.Sk - col0);
   if (off) {
 #pragma unroll
@@ -205,7 +221,7 @@ __device__ __forceinline__ void score_chunk(float* x, int row, int col0, uint32_
 // 700 x 700, head_dim 64, padded: forward 84 -> 46 us, dQ 64 -> 53, dK / dV 124 -> 61 (unmasked 37, 45, 61).
 template <int MSK>
 __device__ __forceinline__ uint32_t dead_keys(const MaskArgs& m, int b, int col0, int lane) {
-  if constexpr (MSK == 0) return 0u;
+  if constexpr (MSK == 0 || MSK == 3) return 0u;
   if (!m.kpm) return 0u;
   const int col = col0 + lane;
   return __ballot_sync(0xffffffffu, col < m.Sk && __ldg(m.kpm + (long long)b * m.kpm_ld + col) != 0);
@@ -398,6 +414,32 @@ __device__ __forceinline__ void umma_rows(uint32_t d, uint32_t a_tmem, uint32_t 
                  (add || kk > 0) ? 1u : 0u);
 }
 
+// =====================================================================================================  window
+// The key blocks that a tile of 128 queries works on: those of its window from block `lo` on, and the `ns` first ones, which hold the
+// sinks (0 where the window reaches into them: then `lo` is 0).  Step i takes block at(i): the first of the window, the sinks, the
+// rest.  So two neighbouring tiles share their steps: the second leaves out the first step if its window begins a block later, and
+// the first the last one.
+struct Keys {
+  int lo, ns, n;
+  __device__ __forceinline__ int at(int i) const { return i == 0 ? lo : i <= ns ? i - 1 : lo + i - ns; }
+};
+__device__ __forceinline__ int window_block(const MaskArgs& m, int tile) {          // the first block of a tile's window
+  return max(0, tile * kBlk + m.ahead - m.window + 1) / kBlk;
+}
+__device__ __forceinline__ int last_block(const MaskArgs& m, int tile) { return (min(tile * kBlk + kBlk, m.Sq) - 1 + m.ahead) / kBlk; }
+__device__ __forceinline__ Keys window_keys(const FlashParams& p, int tile) {
+  const int lo = window_block(p.m, tile);
+  Keys k;
+  k.ns = lo >= p.sink_blocks ? p.sink_blocks : 0;
+  k.lo = lo >= p.sink_blocks ? lo : 0;
+  k.n = k.ns + last_block(p.m, tile) - k.lo + 1;
+  return k;
+}
+// Whether every query of the 128 from q0 on sees all of the 128 keys from k0 on.
+__device__ __forceinline__ bool all_seen(const MaskArgs& m, int q0, int k0) {
+  return k0 + kBlk - 1 <= q0 + m.ahead && (k0 > q0 + kBlk - 1 + m.ahead - m.window || k0 + kBlk <= m.sinks);
+}
+
 // =====================================================================================================  forward
 // Two row tiles a CTA, one warpgroup each (thread = row), so that the softmax of one tile runs under the products of the
 // other: per 128 x 128 block the tensor cores need 1 024 clocks at head_dim 128 and the exponentials 1 024 (16 a clock),
@@ -416,7 +458,10 @@ enum { F_QFULL = 0 /* 2 tiles */, F_QEMPTY = 2 /* 2 */, F_KFULL = 4 /* 2 stages 
 // What blockIdx.x stands for: row tiles g0 (and g0 + 1) of head h of batch entry b, with n0 and n1 steps; nload key blocks in all.
 struct FwdWork {
   int g0, bh, b, h, n0, n1, nload;
+  int s1;                              // window: the second tile's first step
+  Keys keys;
 };
+template <bool WIN>
 __device__ __forceinline__ FwdWork fwd_work(const FlashParams& p, int blk) {
   const int nqb = (p.m.Sq + kBlk - 1) / kBlk, nkb = (p.m.Sk + kBlk - 1) / kBlk, BH = p.B * p.H;
   // row tiles of a piece of work: one or two; heaviest (last) query blocks of a group of heads first
@@ -433,6 +478,17 @@ __device__ __forceinline__ FwdWork fwd_work(const FlashParams& p, int blk) {
   w.bh = grp + blk - level * heads;
   w.b = w.bh / p.H;
   w.h = w.bh - w.b * p.H;
+  w.s1 = 0;
+  if constexpr (WIN) {
+    w.keys = window_keys(p, w.g0);
+    const int nb0 = w.keys.n;
+    const bool two = !p.split && w.g0 + 1 < nqb;
+    w.n0 = p.split ? (nb0 + 1) >> 1 : nb0;
+    w.n1 = p.split ? nb0 >> 1 : two ? nb0 + last_block(p.m, w.g0 + 1) - last_block(p.m, w.g0) : 0;
+    if (two && (w.keys.lo > 0 || p.sink_blocks == 0)) w.s1 = window_block(p.m, w.g0 + 1) - w.keys.lo;
+    w.nload = p.split ? nb0 : max(w.n0, w.n1);
+    return w;
+  }
   const int nb0 = p.m.causal ? min(nkb, w.g0 + 1) : nkb;            // key blocks of the first tile, of the second
   const int nb1 = w.g0 + 1 >= nqb ? 0 : p.m.causal ? min(nkb, w.g0 + 2) : nkb;
   w.n0 = p.split ? (nb0 + 1) >> 1 : nb0;
@@ -445,6 +501,7 @@ template <int HD, int MSK, bool DRP, bool MORE>
 __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_constant__ FlashParams p) {
   constexpr int SUB = HD / 64;
   constexpr int TILE = SUB * kSub;
+  constexpr bool WIN = MSK == 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = sm;                   // 2 tiles (split: the first serves both)
@@ -461,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
   const int counts[23] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 10, 1};
   // The first work is looked up before the wait for the previous kernel: its divisions took 1 000 clocks between set-up and the first
   // copy, of the 12 000 of a launch of one key block (4 x 8 heads of 64 x 64).
-  const FwdWork first = fwd_work(p, (int)blockIdx.x);
+  const FwdWork first = fwd_work<WIN>(p, (int)blockIdx.x);
   asm volatile("" ::"r"(first.b), "r"(first.h), "r"(first.g0), "r"(first.nload));
   const uint32_t tmem = setup_cta(ctl, counts, 23, warp, lane);
   volatile uint32_t* abort_flag = &ctl->abort_flag;
@@ -488,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       auto wait = [&](int i, uint32_t ph) { return mbar_wait(&bar[i], ph, abort_flag, status, tmo); };
       uint32_t n = 0;
       for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, false)) {
-        const FwdWork w = n == 0 ? first : fwd_work(p, blk);
+        const FwdWork w = n == 0 ? first : fwd_work<WIN>(p, blk);
         const int b = w.b, h = w.h;
         const int cq = head_col(p.q, h), ck = head_col(p.k, h), cv = head_col(p.v, h);
         auto load_q = [&](int t) {
@@ -502,10 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
           const int st = nkv & 1;
           const uint32_t ph = (nkv >> 1) & 1u;
           if (!wait(F_KEMPTY + st, ph ^ 1u)) { ok = false; break; }
-          load(F_KFULL + st, ph, sK + st * TILE, &p.mk, p.k_seq1, ck, b, j * kBlk);
+          const int kb = WIN ? w.keys.at(j) : j;
+          load(F_KFULL + st, ph, sK + st * TILE, &p.mk, p.k_seq1, ck, b, kb * kBlk);
           if (j == 0 && !split && w.n1 > 0 && !load_q(1)) { ok = false; break; }
           if (!wait(F_VEMPTY + st, ph ^ 1u)) { ok = false; break; }
-          load(F_VFULL + st, ph, sV + st * TILE, &p.mv, p.v_seq1, cv, b, j * kBlk);
+          load(F_VFULL + st, ph, sV + st * TILE, &p.mv, p.v_seq1, cv, b, kb * kBlk);
         }
         if (!ok) break;
         mbar_arrive(&bar[F_TAKEN]);
@@ -532,31 +590,36 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       };
       uint32_t n = 0, kv0 = 0, np[2] = {0, 0}, nq[2] = {0, 0};      // blocks before this work, P tiles and Q tiles so far
       for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, false)) {
-        const FwdWork w = n == 0 ? first : fwd_work(p, blk);
+        const FwdWork w = n == 0 ? first : fwd_work<WIN>(p, blk);
         const int n0 = w.n0, n1 = w.n1;
         mbar_arrive(&bar[F_TAKEN]);
-        ok = wait(F_QFULL, nq[0]++ & 1u) && issue_s(0, kv0, split || n1 == 0, !split && n0 == 1);
+        const int s1 = WIN ? w.s1 : 0;                    // 1: the second tile has no part in step 0
+        ok = wait(F_QFULL, nq[0]++ & 1u) && issue_s(0, kv0, split || n1 == 0 || s1 > 0, !split && n0 == 1);
         if (ok && n1 > 0) {
           if (!split) ok = wait(F_QFULL + 1, nq[1]++ & 1u);
-          ok = ok && issue_s(1, kv0 + (split ? 1 : 0), true, !split && n1 == 1);
+          if (s1 == 0) ok = ok && issue_s(1, kv0 + (split ? 1 : 0), true, !split && n1 == 1);
         }
         const int nmax = max(n0, n1);
         for (int i = 0; i < nmax && ok; ++i) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const int nt = t ? n1 : n0;
+            const int nt = t ? n1 : n0, begin = t ? s1 : 0;
             if (!ok || i >= nt) continue;
+            if (WIN && i < begin) {                      // its first S comes after the other tile's S of the same block
+              ok = issue_s(1, kv0 + begin, true, n1 == begin + 1);
+              continue;
+            }
             const uint32_t c = kv0 + (split ? 2 * i + t : i);
             const int st = c & 1;
             // the block's second tile releases it; a tile that is done no longer counts
-            const bool last = split || t == 1 || i >= n1;
+            const bool last = split || t == 1 || i >= n1 || i < s1;
             const uint32_t pp = np[t]++ & 1u;
             if (!wait(F_VFULL + st, (c >> 1) & 1u) || !wait(F_PFULL + t, pp)) { ok = false; break; }
             tc_fence_after();
             const uint32_t vb = aV + st * TILE, pt = tmem + (uint32_t)(t * 128), d = tmem + (uint32_t)(256 + t * HD);
 #pragma unroll
             for (int kk = 0; kk < 6; ++kk)
-              umma_bf16_ts(d, pt + kk * 8, make_smem_desc(vb + kk * 2048, kSub, 1024), id_o, (i > 0 || kk > 0) ? 1u : 0u);
+              umma_bf16_ts(d, pt + kk * 8, make_smem_desc(vb + kk * 2048, kSub, 1024), id_o, (i > begin || kk > 0) ? 1u : 0u);
             if (!wait(F_PTAIL + t, pp)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
@@ -587,14 +650,15 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
     // stamps of the two tiles' first warps of CTA 0: [warp 0 | warp 4][step < 16][event < 8]
     long long* tr = (p.trace && blockIdx.x == 0 && lane == 0 && (warp & 3) == 0) ? p.trace + (warp >> 2) * 128 : nullptr;
     for (int blk = (int)blockIdx.x; blk >= 0; blk = following(n++, true)) {
-    const FwdWork w = n == 0 ? first : fwd_work(p, blk);
+    const FwdWork w = n == 0 ? first : fwd_work<WIN>(p, blk);
     if (lane == 0) mbar_arrive(&bar[F_TAKEN]);
     const int bh = w.bh, b = w.b, h = w.h, n1 = w.n1;
     const int nt = t ? n1 : w.n0, gt = w.g0 + (split ? 0 : t);
     const int row = gt * kBlk + rt;
     float m_used = -INFINITY, l = 0.f;
-    for (int i = 0; i < nt; ++i, ++ns) {
-      const int c = split ? 2 * i + t : i, col0 = c * kBlk;
+    const int begin = WIN && t ? w.s1 : 0;
+    for (int i = begin; i < nt; ++i, ++ns) {
+      const int step = split ? 2 * i + t : i, c = WIN ? w.keys.at(step) : step, col0 = c * kBlk;
       if (tr && ns < 16) tr[ns * 8 + 0] = clock64();
       uint32_t dead[4];
 #pragma unroll
@@ -605,8 +669,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       if (tr && ns < 16) tr[ns * 8 + 1] = clock64();
       // A block that needs more than the scale is put right in TMEM first, 32 or 64 columns at a time, so that the loop below is one
       // for all blocks; one that only needs the scale keeps the raw scores: the scale rides in the exponent's multiply-add.
-      const bool plain = MSK != 2 && !(dead[0] | dead[1] | dead[2] | dead[3]) && !(M.causal && c == gt) && (col0 + kBlk <= M.Sk) &&
-                         M.scale_log2 >= 0.f;          // the maximum commutes with a positive scale only
+      const bool unmasked = WIN ? all_seen(M, gt * kBlk, col0)
+                                : MSK != 2 && !(dead[0] | dead[1] | dead[2] | dead[3]) && !(M.causal && c == gt);
+      const bool plain = unmasked && (col0 + kBlk <= M.Sk) && M.scale_log2 >= 0.f;   // the maximum commutes with a positive scale only
       if (!plain) {
         constexpr int NQ = MSK == 2 ? 1 : 2;           // chunks at a time: the additive mask's code is long
 #pragma unroll 1
@@ -644,8 +709,8 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       // a -inf below a finite maximum gets 2^-126 beside 2^-8 or more.
       const bool fin = fabsf(mx) < INFINITY;
       bool some = !DRP && plain;
-      if (__any_sync(0xffffffffu, (i > 0 && need) || !fin)) {
-        if (i > 0 && __any_sync(0xffffffffu, need)) {
+      if (__any_sync(0xffffffffu, (i > begin && need) || !fin)) {
+        if (i > begin && __any_sync(0xffffffffu, need)) {
           // the S that was waited for came after the P V of the tile's previous step: O is complete up to there
           const float alpha = need ? ex2_approx(m_used - cand) : 1.f;
 #pragma unroll
@@ -824,8 +889,60 @@ enum { B_FULL = 0, B_EMPTY = 7, B_STAT = 14 /* 2 */, B_SFULL = 16 /* 2 */, B_PFU
 // What blockIdx.x stands for: the key block kb, or (kb < 0) the query block qb, of head h of batch entry b.
 struct BwdWork {
   int kb, qb, bh, b, h;
+  // window: dK / dV take the query blocks q0 .. q0 + nq - 1 of `qpk` heads from h on, steps s0 .. s0 + n - 1 of those; `piece`: where
+  // they leave fp32 sums (-1: in dK and dV)
+  int q0, nq, s0, n, piece;
+  Keys keys;                           // dQ
 };
+// Window: the blocks of sinks first, whose queries are all there are, in p.pieces pieces each; then for every key head the other key
+// blocks and behind them, as they are `qpk` times as short, the query blocks of its heads.
+__device__ __forceinline__ BwdWork window_work(const FlashParams& p, int blk) {
+  const MaskArgs& m = p.m;
+  const int nq = (m.Sq + kBlk - 1) / kBlk, nk = (m.Sk + kBlk - 1) / kBlk, heads_k = p.H / p.qpk, BK = p.B * heads_k;
+  BwdWork w = {-1, -1, 0, 0, 0, 0, 0, 0, 0, -1, {0, 0, 0}};
+  int pair, of = 0, pieces = 1;                             // pair: (batch, key head)
+  const int sink_work = BK * p.sink_blocks * p.pieces;
+  if (blk < sink_work) {
+    of = blk / (BK * p.sink_blocks);
+    blk -= of * BK * p.sink_blocks;
+    pair = blk / p.sink_blocks;
+    w.kb = blk - pair * p.sink_blocks;
+    pieces = p.pieces;
+    if (p.part) w.piece = (pair * p.sink_blocks + w.kb) * pieces + of;
+  } else {
+    blk -= sink_work;
+    const int nkb = nk - p.first_block, per = nkb + nq * p.qpk, span = p.group * per;
+    const int g = blk / span, grp = g * p.group, heads = min(p.group, BK - grp);
+    blk -= g * span;
+    const int row = blk / heads;
+    pair = grp + blk - row * heads;
+    if (row < nkb) w.kb = p.first_block + row;
+    else {
+      const int r = row - nkb;
+      w.qb = nq - 1 - r / p.qpk;
+      w.h = r % p.qpk;
+    }
+  }
+  w.b = pair / heads_k;
+  w.h += (pair - w.b * heads_k) * p.qpk;
+  w.bh = w.b * p.H + w.h;
+  if (w.kb >= 0) {
+    w.q0 = max(0, w.kb * kBlk - m.ahead) / kBlk;
+    // the last query that sees the block's last key; a sink is seen to the end
+    const long long last = (long long)w.kb * kBlk + kBlk - 2 + m.window - m.ahead;
+    w.nq = (w.kb < p.sink_blocks ? nq : (int)min((long long)nq, last / kBlk + 1)) - w.q0;
+    const int all = w.nq * p.qpk;
+    w.s0 = (int)((long long)all * of / pieces);
+    w.n = (int)((long long)all * (of + 1) / pieces) - w.s0;
+  } else {
+    w.keys = window_keys(p, w.qb);
+    w.n = w.keys.n;
+  }
+  return w;
+}
+template <bool WIN>
 __device__ __forceinline__ BwdWork bwd_work(const FlashParams& p, int blk) {
+  if constexpr (WIN) return window_work(p, blk);
   const int nq = (p.m.Sq + kBlk - 1) / kBlk, nk = (p.m.Sk + kBlk - 1) / kBlk, BH = p.B * p.H, both = min(nq, nk), span = p.group * (nq + nk);
   // a group of heads: a key block of each, a query block of each and so on, the longest first (causal: first keys, last queries), then
   // what one kind has more
@@ -836,7 +953,7 @@ __device__ __forceinline__ BwdWork bwd_work(const FlashParams& p, int blk) {
     blk -= g * span;
   }
   const int heads = min(p.group, BH - grp), row = blk / heads;
-  BwdWork w = {-1, -1, grp + blk - row * heads, 0, 0};
+  BwdWork w = {-1, -1, grp + blk - row * heads, 0, 0, 0, 0, 0, 0, -1, {0, 0, 0}};
   if (row < 2 * both) { if (row & 1) w.qb = nq - 1 - (row >> 1); else w.kb = row >> 1; }
   else if (nk > nq) w.kb = row - both;
   else w.qb = nq - 1 + both - row;
@@ -850,6 +967,7 @@ constexpr int kBwdSlack = 768;          // all that a CTA's shared memory leaves
 template <int HD, int MSK, bool DRP, bool MORE, bool ONE = false>
 __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_constant__ FlashParams p) {
   constexpr int TILE = (HD / 64) * kSub;
+  constexpr bool WIN = MSK == 3;
   extern __shared__ __align__(1024) uint8_t smem_tiles[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_tiles) + 1023) & ~uintptr_t(1023));
   if (sm - smem_tiles > kBwdSlack) {
@@ -864,7 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
   // counts by barrier index: copies and commits 1; statistics 32 (lanes); P and dS, accumulators read 8 (one per row warp); next work
   // 1 and 10 (producer, issuer, eight row warps)
   const int counts[26] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 32, 32, 1, 1, 8, 1, 8, 1, 8, 1, 10, 1};
-  const BwdWork first = bwd_work(p, (int)blockIdx.x);       // before the wait for the previous kernel, as in forward
+  const BwdWork first = bwd_work<WIN>(p, (int)blockIdx.x);       // before the wait for the previous kernel, as in forward
   asm volatile("" ::"r"(first.b), "r"(first.h), "r"(first.kb), "r"(first.qb));
   const uint32_t tmem = setup_cta(ctl, counts, 26, warp, lane);
   volatile uint32_t* abort_flag = &ctl->abort_flag;
@@ -895,19 +1013,19 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
       return true;
     };
     for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, true)) {
-      const BwdWork w = n == 0 ? first : bwd_work(p, blk);
+      const BwdWork w = n == 0 ? first : bwd_work<WIN>(p, blk);
       const int b = w.b, h = w.h;
       const int cq = head_col(p.q, h), ck = head_col(p.k, h), cv = head_col(p.v, h), cg = head_col(p.dout, h);
       if (w.kb >= 0) {
-        const long long base = (long long)w.bh * M.Sq;
-        const int i0 = M.causal ? w.kb : 0;
+        const int i0 = WIN ? w.s0 : M.causal ? w.kb : 0, i1 = WIN ? w.s0 + w.n : nqb;
         ok = load(0, &p.mk, p.k_seq1, ck, b, w.kb * kBlk);
-        for (int i = i0; i < nqb && ok; ++i) {
-          const int st = (i - i0) & 1, q0 = i * kBlk;
-          ok = load(2 + st, &p.mq, p.q_seq1, cq, b, q0);
+        for (int i = i0; i < i1 && ok; ++i) {
+          const int st = (i - i0) & 1, hq = WIN ? i / w.nq : 0, q0 = (WIN ? w.q0 + i - hq * w.nq : i) * kBlk;
+          const long long base = (long long)(w.bh + hq) * M.Sq;
+          ok = load(2 + st, &p.mq, p.q_seq1, WIN ? head_col(p.q, h + hq) : cq, b, q0);
           if (!ok) break;
           if (i == i0) ok = load(1, &p.mv, p.v_seq1, cv, b, w.kb * kBlk);
-          ok = ok && load(4 + st, &p.mdo, p.do_seq1, cg, b, q0);
+          ok = ok && load(4 + st, &p.mdo, p.do_seq1, WIN ? head_col(p.dout, h + hq) : cg, b, q0);
           float* stat = sStat + st * 2 * kBlk;          // free with its Q tile: dK read that after the rows had read these
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -918,12 +1036,13 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           mbar_arrive(&bar[B_STAT + st]);
         }
       } else {
-        const int nb = M.causal ? min(nkb, w.qb + 1) : nkb;
+        const int nb = WIN ? w.n : M.causal ? min(nkb, w.qb + 1) : nkb;
         ok = load(0, &p.mq, p.q_seq1, cq, b, w.qb * kBlk);
         for (int j = 0; j < nb && ok; ++j) {
-          ok = load(2 + j % 3, &p.mk, p.k_seq1, ck, b, j * kBlk);
+          const int kb = WIN ? w.keys.at(j) : j;
+          ok = load(2 + j % 3, &p.mk, p.k_seq1, ck, b, kb * kBlk);
           if (ok && j == 0) ok = load(1, &p.mdo, p.do_seq1, cg, b, w.qb * kBlk);
-          ok = ok && load(5 + (j & 1), &p.mv, p.v_seq1, cv, b, j * kBlk);
+          ok = ok && load(5 + (j & 1), &p.mv, p.v_seq1, cv, b, kb * kBlk);
         }
       }
       if (!ok) break;
@@ -958,11 +1077,11 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
         return true;
       };
       for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, false)) {
-        const BwdWork w = n == 0 ? first : bwd_work(p, blk);
+        const BwdWork w = n == 0 ? first : bwd_work<WIN>(p, blk);
         mbar_arrive(&bar[B_TAKEN]);
         const uint32_t read = (n & 1u) ^ 1u;            // the accumulators of the work before have been read out
         if (w.kb >= 0) {
-          const int nit = nqb - (M.causal ? w.kb : 0);
+          const int nit = WIN ? w.n : nqb - (M.causal ? w.kb : 0);
           ok = tile(0) && product(tS, 0, 2, B_SFULL, nit == 1, false) && tile(1) && product(tP, 1, 4, B_DPFULL, nit == 1, false) &&
                wait(B_ACCREAD, read);
           for (int it = 0; it < nit && ok; ++it) {
@@ -987,7 +1106,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
             else umma_commit(&bar[B_ACC]);
           }
         } else {
-          const int nb = M.causal ? min(nkb, w.qb + 1) : nkb;
+          const int nb = WIN ? w.n : M.causal ? min(nkb, w.qb + 1) : nkb;
           auto issue_s = [&](int j) {
             return product(j & 1 ? tmem + 384 : tS, 0, 2 + j % 3, B_SFULL + (j & 1), j + 1 == nb, false);
           };
@@ -1022,19 +1141,20 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
     auto wait = [&](int i, uint32_t ph) { return warp_wait(&bar[i], ph, abort_flag, status, tmo); };
     long long* tr = (p.trace && blockIdx.x == 0 && lane == 0 && (warp & 3) == 0) ? p.trace + (warp >> 2) * 128 : nullptr;
     for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, true)) {
-      const BwdWork w = n == 0 ? first : bwd_work(p, blk);
+      const BwdWork w = n == 0 ? first : bwd_work<WIN>(p, blk);
       if (lane == 0) mbar_arrive(&bar[B_TAKEN]);
       const int bh = w.bh, b = w.b, h = w.h;
       if (w.kb >= 0) {
-        const int k0 = w.kb * kBlk, i0 = M.causal ? w.kb : 0, nit = nqb - i0;
+        const int k0 = w.kb * kBlk, i0 = WIN ? w.s0 : M.causal ? w.kb : 0, nit = WIN ? w.n : nqb - i0;
         const uint32_t aS = tS + lane_off + (uint32_t)(wg * 64);
         const int key = k0 + rt;
         bool key_dead = key >= M.Sk;
-        if constexpr (MSK != 0) key_dead = key_dead || (M.kpm && __ldg(M.kpm + (long long)b * M.kpm_ld + key));
+        if constexpr (MSK == 1 || MSK == 2) key_dead = key_dead || (M.kpm && __ldg(M.kpm + (long long)b * M.kpm_ld + key));
         const bool keys_plain = MSK != 2 && !__any_sync(0xffffffffu, key_dead);
         for (int it = 0; it < nit; ++it) {
           const int st = it & 1;
-          const int qbase = (i0 + it) * kBlk + wg * 64;          // first query of this thread
+          const int qb = WIN ? w.q0 + (i0 + it) % w.nq : i0 + it;
+          const int qbase = qb * kBlk + wg * 64;                 // first query of this thread
           const float* nlse = sStat + st * 2 * kBlk + wg * 64;
           const float* ndel = nlse + kBlk;
           // Dropout bits.  One generator call covers four neighbouring keys, which sit in four neighbouring lanes: each lane
@@ -1070,7 +1190,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           tmem_ld32f(aS, x);
           tmem_ld32f(aS + 32, x + 32);
           tmem_ld_wait();
-          if (keys_plain && !(M.causal && it == 0)) {            // the diagonal crosses a causal key block's first query block
+          if (keys_plain && (WIN ? all_seen(M, qb * kBlk, k0) : !(M.causal && it == 0))) {      // the diagonal crosses a causal key block's first query block
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
               const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, make_float2(nl[i], nl[i + 1]));
@@ -1088,7 +1208,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
                                      : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(M.mask) + mi))) * kLog2e;
                 }
               }
-              x[i] = key_dead || (M.causal && key > q) ? -INFINITY : xs + nl[i];
+              bool hidden = M.causal && key > q;
+              if constexpr (WIN) hidden = key > q + M.ahead || (key <= q + M.ahead - M.window && key >= M.sinks);
+              x[i] = key_dead || hidden ? -INFINITY : xs + nl[i];
             }
           }
 #pragma unroll
@@ -1142,14 +1264,14 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           if (tr && it < 16) tr[it * 8 + 4] = clock64();
         }
       } else {
-        const int q0 = w.qb * kBlk, nb = M.causal ? min(nkb, w.qb + 1) : nkb;
+        const int q0 = w.qb * kBlk, nb = WIN ? w.n : M.causal ? min(nkb, w.qb + 1) : nkb;
         const int row = q0 + rt;
         const bool live = row < M.Sq;
         const float nlse = live ? -__ldg(p.lse + (long long)bh * M.Sq + row) : -INFINITY;
         const float ndel = live ? -__ldg(p.delta + (long long)bh * M.Sq + row) : 0.f;
         const float2 nl = make_float2(nlse, nlse), nd = make_float2(ndel, ndel);
         for (int j = 0; j < nb; ++j) {
-          const int col0 = j * kBlk + wg * 64;
+          const int kb = WIN ? w.keys.at(j) : j, col0 = kb * kBlk + wg * 64;
           const uint32_t dead[2] = {dead_keys<MSK>(M, b, col0, lane), dead_keys<MSK>(M, b, col0 + 32, lane)};
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if constexpr (DRP) {
@@ -1164,7 +1286,8 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           tmem_ld32f(aS, x);
           tmem_ld32f(aS + 32, x + 32);
           tmem_ld_wait();
-          const bool plain = MSK != 2 && !(dead[0] | dead[1]) && !(M.causal && j == w.qb) && (j * kBlk + kBlk <= M.Sk);
+          const bool unmasked = WIN ? all_seen(M, q0, kb * kBlk) : MSK != 2 && !(dead[0] | dead[1]) && !(M.causal && j == w.qb);
+          const bool plain = unmasked && (kb * kBlk + kBlk <= M.Sk);
           if (plain) {
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
@@ -1210,7 +1333,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
         const bool is_q = w.kb < 0 || (ONE && a == 2);
         const DRef& out = is_q ? p.dq : a ? p.dk : p.dv;
         const int left = (is_q ? M.Sq : M.Sk) - r0;
-        __nv_bfloat16* dst = row_ptr(out, b, r0, h) + wg * (HD / 2);
+        __nv_bfloat16* dst = row_ptr(out, b, r0, WIN && !is_q ? h / p.qpk : h) + wg * (HD / 2);
         const float mul = !is_q && a == 0 ? 1.f : M.sm_scale;
         const uint32_t acc = ONE && a == 2 ? tS : tAcc + (uint32_t)(a * HD);
 #pragma unroll
@@ -1225,12 +1348,43 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= mul;
-          store_rows32(dst + c * 32, out.ss, left, o, lane);
+          if (WIN && w.piece >= 0) {     // [piece][dV, dK][HD / 4][key][4]: the lanes of a store side by side
+            float4* sum = reinterpret_cast<float4*>(p.part) + ((long long)w.piece * 2 + a) * (HD / 4) * kBlk + (wg * (HD / 8) + c * 8) * kBlk + rt;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i * kBlk] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            store_rows32(dst + c * 32, out.ss, left, o, lane);
+          }
         }
       }
     }
   }
   teardown_cta(tmem, warp);
+}
+
+// The sums that the pieces of a block of sinks left, added up in their order: one thread for four columns of dV or dK of a key.
+template <int HD>
+__global__ void __launch_bounds__(256) flash_sinks_kernel(const float* __restrict__ part, DRef dk, DRef dv, int Sk, int heads_k,
+                                                          int sink_blocks, int pieces, long long items) {
+  pdl_prologue();
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= items) return;
+  constexpr int PER = 2 * (HD / 4) * kBlk;                  // items of a block of keys, in the order of the sums
+  const long long blk = i / PER;
+  const int e = (int)(i - blk * PER);
+  const float4* src = reinterpret_cast<const float4*>(part) + blk * pieces * PER + e;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < pieces; ++k) {
+    const float4 v = __ldcs(src + (long long)k * PER);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const int kb = (int)(blk % sink_blocks), key = kb * kBlk + e % kBlk, col = e / kBlk % (HD / 4) * 4;
+  if (key >= Sk) return;
+  const long long pair = blk / sink_blocks;
+  const DRef& r = e / kBlk >= HD / 4 ? dk : dv;
+  *reinterpret_cast<uint2*>(row_ptr(r, (int)(pair / heads_k), key, (int)(pair % heads_k)) + col) =
+      make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
 }
 
 // =====================================================================================================  parts
@@ -1258,13 +1412,14 @@ cudaError_t launch_flash(const FlashParams& P, int grid, int smem, cudaStream_t 
   (kind == 1 ? launch_flash<flash_fwd_kernel<HD, MSK, DRP, true>>(P, grid, smem_fwd(HD), (cudaStream_t)stream)          \
              : launch_flash<flash_fwd_kernel<HD, MSK, DRP, false>>(P, grid, smem_fwd(HD), (cudaStream_t)stream))
 #define RTP_FLASH_BWD(HD, MSK, DRP)                                                                                     \
-  (kind == 2   ? launch_flash<flash_bwd_kernel<HD, MSK, DRP, false, true>>(P, grid, smem_bwd(HD), (cudaStream_t)stream) \
+  (kind == 2 && MSK != 3 ? launch_flash<flash_bwd_kernel<HD, MSK == 3 ? 0 : MSK, DRP, false, true>>(P, grid, smem_bwd(HD), (cudaStream_t)stream) \
    : kind == 1 ? launch_flash<flash_bwd_kernel<HD, MSK, DRP, true>>(P, grid, smem_bwd(HD), (cudaStream_t)stream)        \
                : launch_flash<flash_bwd_kernel<HD, MSK, DRP, false>>(P, grid, smem_bwd(HD), (cudaStream_t)stream))
 #define RTP_FLASH_PART_FN(NAME, LAUNCH, HD)                                                              \
   extern "C" int NAME(const void* params, int mask, int drp, int kind, int grid, void* stream) {         \
     const FlashParams& P = *reinterpret_cast<const FlashParams*>(params);                                \
-    return (int)(mask == 2   ? (drp ? LAUNCH(HD, 2, true) : LAUNCH(HD, 2, false))                        \
+    return (int)(mask == 3   ? LAUNCH(HD, 3, false)                                                      \
+                 : mask == 2 ? (drp ? LAUNCH(HD, 2, true) : LAUNCH(HD, 2, false))                        \
                  : mask == 1 ? (drp ? LAUNCH(HD, 1, true) : LAUNCH(HD, 1, false))                        \
                              : (drp ? LAUNCH(HD, 0, true) : LAUNCH(HD, 0, false)));                      \
   }
@@ -1383,6 +1538,36 @@ int fill_common(const RtpFlashArgs* a, FlashParams& P) {
   P.q = dref(a->q); P.k = dref(a->k); P.v = dref(a->v); P.o = dref(a->o);
   return 0;
 }
+// What the window kernels need beside the common part.
+int fill_window(const RtpWindowArgs* w, FlashParams& P) {
+  const RtpFlashArgs& a = w->f;
+  if (a.causal || a.mask || a.kpm || a.drop_p != 0.f) return ffail("window attention: no other mask and no dropout");
+  if (w->kv_heads <= 0 || a.H % w->kv_heads) return ffail("window attention: the query heads must be a multiple of the key heads");
+  if (a.Sq > a.Sk) return ffail("window attention: more queries than keys");
+  if (w->window < 1 || w->sinks < 0) return ffail("window attention: a window of at least one key, no negative number of sinks");
+  if (fill_common(&a, P)) return -1;
+  P.m.window = std::min(w->window, a.Sk);
+  P.m.sinks = std::min(w->sinks, a.Sk);
+  P.m.ahead = a.Sk - a.Sq;
+  P.qpk = a.H / w->kv_heads;
+  P.sink_blocks = (P.m.sinks + kBlk - 1) / kBlk;
+  P.first_block = std::max(P.sink_blocks, std::max(0, P.m.ahead - P.m.window + 1) / kBlk);
+  P.pieces = 1;
+  P.part = nullptr;
+  return 0;
+}
+// Pieces that the queries of a block of sinks fall into.  All queries see a sink: over a long context its block would be many times
+// the work of any other key block (32768 queries, window 2048: 15 times), and while it lasts the rest runs out.  So it is cut into
+// pieces as long as the others, as long as those are no more than fill the SMs twice.
+int sink_pieces(const RtpWindowArgs* w, int sms) {
+  const RtpFlashArgs& a = w->f;
+  const long long sinks = std::min(w->sinks, a.Sk), blocks = (sinks + kBlk - 1) / kBlk, qpk = a.H / w->kv_heads;
+  if (!blocks) return 1;
+  const long long nq = (a.Sq + kBlk - 1) / kBlk, first = std::max(0ll, (blocks - 1) * kBlk - (a.Sk - a.Sq)) / kBlk;
+  const long long all = (nq - first) * qpk, other = std::max(8ll, (std::min(w->window, a.Sk) / kBlk + 2) * qpk);
+  const long long room = std::max(1ll, 2ll * sms / (blocks * a.B * w->kv_heads));
+  return (int)std::max(1ll, std::min({all / other, room, all}));
+}
 int mask_kind(const RtpFlashArgs* a) { return a->mask ? 2 : a->kpm ? 1 : 0; }
 int launched(int e, const char* what) { return e == (int)cudaSuccess ? 0 : ffail(std::string(what) + ": " + cudaGetErrorString((cudaError_t)e)); }
 
@@ -1432,6 +1617,63 @@ int rtp_flash_bwd(const RtpFlashArgs* a, void* stream) {
   if (e != cudaSuccess) return ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
   return launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, mask_kind(a), P.m.thresh != 0, kind, grid, stream),
                   "flash_bwd");
+}
+
+int rtp_window_fwd(const RtpWindowArgs* w, void* stream) {
+  static thread_local FlashParams P;
+  if (fill_window(w, P)) return -1;
+  const RtpFlashArgs* a = &w->f;
+  const int tiles = (a->Sq + kBlk - 1) / kBlk, BH = a->B * a->H;
+  P.split = (long long)tiles * BH <= device_sms();              // as without a window
+  // whole groups of heads that share their keys
+  const int g = head_group(4ll * std::min(a->Sk, P.m.window + 2 * kBlk) * a->head_dim, BH);
+  P.group = std::min(BH, std::max(P.qpk, g / P.qpk * P.qpk));
+  const int grid = (P.split ? tiles : (tiles + 1) / 2) * BH;
+  return launched((a->head_dim == 64 ? rtp_flash_part_fwd64 : rtp_flash_part_fwd128)(&P, 3, 0, grid > device_sms(), grid, stream),
+                  "window_fwd");
+}
+
+unsigned long long rtp_window_bwd_scratch(const RtpWindowArgs* w) {
+  if (w->kv_heads <= 0 || w->f.H % w->kv_heads || w->f.Sq > w->f.Sk) return 0;      // the launch will say so
+  const int n = sink_pieces(w, device_sms());
+  const unsigned long long blocks = (unsigned long long)((std::min(w->sinks, w->f.Sk) + kBlk - 1) / kBlk) * w->f.B * w->kv_heads;
+  return n > 1 ? blocks * n * 2 * kBlk * w->f.head_dim * sizeof(float) : 0;
+}
+
+int rtp_window_bwd(const RtpWindowArgs* w, void* stream) {
+  static thread_local FlashParams P;
+  if (fill_window(w, P)) return -1;
+  const RtpFlashArgs* a = &w->f;
+  if (!a->lse || !a->delta) return ffail("window attention backward: lse and delta buffers required");
+  if (check_ref(a->dout, "dout", a->head_dim) || check_ref(a->dq, "dq", a->head_dim) || check_ref(a->dk, "dk", a->head_dim) ||
+      check_ref(a->dv, "dv", a->head_dim))
+    return -1;
+  if (make_map3(&P.mdo, &P.do_seq1, a->dout, a->B, a->Sq, "dout")) return -1;
+  P.dout = dref(a->dout); P.dq = dref(a->dq); P.dk = dref(a->dk); P.dv = dref(a->dv);
+  const unsigned long long need = rtp_window_bwd_scratch(w);
+  if (need) {
+    if (!w->scratch || w->scratch_bytes < need || (reinterpret_cast<uintptr_t>(w->scratch) & 15))
+      return ffail("window attention backward: workspace missing, too small or not aligned to 16 bytes");
+    P.part = reinterpret_cast<float*>(w->scratch);
+    P.pieces = sink_pieces(w, device_sms());
+  }
+  const int nq = (a->Sq + kBlk - 1) / kBlk, nk = (a->Sk + kBlk - 1) / kBlk, BK = a->B * w->kv_heads;
+  const long long grid = (long long)BK * (P.sink_blocks * P.pieces + nk - P.first_block + (long long)nq * P.qpk);
+  if (grid > 0x7fffffffll) return ffail("window attention backward: problem too large");
+  P.group = head_group(4ll * (std::min(a->Sq, P.m.window) * (long long)P.qpk + std::min(a->Sk, P.m.window)) * a->head_dim, BK);
+  cudaStream_t s = (cudaStream_t)stream;
+  const long long rows = (long long)a->B * a->Sq * a->H, per = 256 / (a->head_dim / 8);
+  cudaError_t e = launch_k(a->head_dim == 64 ? flash_delta_kernel<64> : flash_delta_kernel<128>,
+                           dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
+  if (e != cudaSuccess) return ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
+  if (launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, 3, 0, grid > 2 * device_sms(), (int)grid, stream),
+               "window_bwd"))
+    return -1;
+  if (!P.part) return 0;
+  const long long items = (long long)BK * P.sink_blocks * 2 * (a->head_dim / 4) * kBlk;
+  e = launch_k(a->head_dim == 64 ? flash_sinks_kernel<64> : flash_sinks_kernel<128>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0,
+               s, (const float*)P.part, P.dk, P.dv, a->Sk, w->kv_heads, P.sink_blocks, P.pieces, items);
+  return e == cudaSuccess ? 0 : ffail(std::string("flash_sinks: ") + cudaGetErrorString(e));
 }
 
 }  // extern "C"

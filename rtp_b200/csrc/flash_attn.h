@@ -39,6 +39,23 @@ typedef struct {
   unsigned long long* status;   // device status word (0 = ok; a bounded wait that ran out writes its code)
 } RtpFlashArgs;
 
+// Causal attention over a window of keys and the first few (sinks): query i stands at position p = i + Sk - Sq and sees key j if
+// j <= p and (j > p - window or j < sinks).  H query heads share kv_heads key and value heads: head h reads k and v at
+// its col(h), which a group of neighbours has in common (hpg = H / kv_heads, hstride = 0); dk and dv have kv_heads heads.
+// f.causal, f.mask, f.kpm and f.drop_p are zero.  f.lse may be null in a forward without a backward.
+typedef struct {
+  RtpFlashArgs f;
+  int kv_heads, window, sinks;
+  // Backward: rtp_window_bwd_scratch() bytes (0: none), 16-byte aligned, the launch's own until it is over.
+  void* scratch;
+  unsigned long long scratch_bytes;
+} RtpWindowArgs;
+int rtp_window_fwd(const RtpWindowArgs* a, void* stream);
+unsigned long long rtp_window_bwd_scratch(const RtpWindowArgs* a);
+// delta, then dQ and dK / dV, then (with a workspace) the sums of the sinks' gradients.  Rows of dk and dv of whole blocks of 128 keys
+// that no query sees are not written.
+int rtp_window_bwd(const RtpWindowArgs* a, void* stream);
+
 int rtp_flash_fwd(const RtpFlashArgs* a, void* stream);
 int rtp_flash_bwd(const RtpFlashArgs* a, void* stream);   // two launches: delta, then dQ and dK / dV
 const char* rtp_flash_last_error(void);

@@ -134,6 +134,11 @@ class FlashArgs(C.Structure):
     ]
 
 
+class WindowArgs(C.Structure):
+    _fields_ = [("f", FlashArgs), ("kv_heads", C.c_int), ("window", C.c_int), ("sinks", C.c_int), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_ulonglong)]
+
+
 class ReduceBlocks(C.Structure):
     _fields_ = [("src", C.c_void_p), ("block_elems", C.c_longlong), ("out", C.c_void_p)]
 
@@ -202,6 +207,10 @@ def lib():
         L.rtp_flash_fwd.argtypes = [C.POINTER(FlashArgs), C.c_void_p]
         L.rtp_flash_bwd.argtypes = [C.POINTER(FlashArgs), C.c_void_p]
         L.rtp_flash_last_error.restype = C.c_char_p
+        L.rtp_window_fwd.argtypes = [C.POINTER(WindowArgs), C.c_void_p]
+        L.rtp_window_bwd.argtypes = [C.POINTER(WindowArgs), C.c_void_p]
+        L.rtp_window_bwd_scratch.argtypes = [C.POINTER(WindowArgs)]
+        L.rtp_window_bwd_scratch.restype = C.c_ulonglong
         L.rtp_linear_fwd_emu.argtypes = [C.POINTER(Ring), C.POINTER(LinearFwd), C.c_int, C.c_void_p]
         L.rtp_linear_bwd_emu.argtypes = [C.POINTER(Ring), C.POINTER(LinearBwd), C.c_int, C.c_void_p]
         L.rtp_linear_bwd_folds_bias.argtypes = [C.POINTER(Ring), C.POINTER(LinearBwd)]

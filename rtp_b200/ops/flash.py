@@ -226,3 +226,120 @@ def flash_attention_packed(qkv, B, S, H, nshard=1, seq_first=False, causal=False
         offset = next_dropout_offset()
     return _FlashPackedFn.apply(qkv, B, S, H, nshard, bool(seq_first), bool(causal), attn_mask, key_padding_mask,
                                 float(dropout_p), seed, offset or 0, step)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# causal attention over a window and sinks
+# ---------------------------------------------------------------------------------------------------------------------
+def check_window_args(q, k, v, window, sinks):
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"window attention: q must be [B, Sq, H, hd], k and v [B, Sk, Hk, hd], got {tuple(q.shape)}, {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+        raise ValueError("window attention: q, k and v must have the same type and device")
+    if not q.dtype.is_floating_point:
+        raise ValueError(f"window attention: floating-point tensors only, got {q.dtype}")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"window attention: the query heads must be a multiple of the key heads, got {q.shape[2]} and {k.shape[2]}")
+    if q.shape[1] > k.shape[1]:
+        raise ValueError(f"window attention: the queries are the last ones of the keys' sequence, got {q.shape[1]} queries and {k.shape[1]} keys")
+    for name, n, least in (("window", window, 1), ("sinks", sinks, 0)):
+        if isinstance(n, bool) or not isinstance(n, int) or n < least:
+            raise ValueError(f"window attention: {name} must be an int of at least {least}, got {n!r}")
+
+
+def _addressable(t):
+    """``t``, or a copy that the copies of tiles can address: unit stride inside a head, other strides multiples of 16 bytes and not
+    zero, columns of a row (all heads) within 32 bits."""
+    sb, ss, sh, sd = t.stride()
+    B, S, H, hd = t.shape
+    if sd == 1 and not (sb | ss | sh) & 7 and (sb or B == 1) and (ss or S == 1) and t.data_ptr() % 16 == 0 and (H - 1) * sh + hd < 1 << 31:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)      # also of a contiguous tensor at an odd address
+
+
+def _shared_ref(t, group):
+    """FlashRef of a [B, S, Hk, hd] view whose heads serve ``group`` query heads each."""
+    _, _, H, hd = t.shape
+    sb, ss, sh, _ = t.stride()
+    return _lib.FlashRef(t.data_ptr(), sb, ss, (H - 1) * sh + hd, 0, group, sh, 0)
+
+
+def _window_args(q, k, v, o, lse, window, sinks, sm_scale):
+    B, Sq, H, hd = q.shape
+    Sk, Hk = k.shape[1:3]
+    a = _lib.WindowArgs()
+    f, most = a.f, 2 ** 31 - 1
+    f.q, f.o, f.k, f.v = _ref4(q), _ref4(o), _shared_ref(k, H // Hk), _shared_ref(v, H // Hk)
+    f.lse = lse.data_ptr() if lse is not None else None
+    f.B, f.H, f.Sq, f.Sk, f.head_dim, f.sm_scale = B, H, Sq, Sk, hd, sm_scale
+    f.status = _lib.status_word(q.device).data_ptr()
+    a.kv_heads, a.window, a.sinks = Hk, min(window, most), min(sinks, most)
+    return a
+
+
+def _window_check(rc, what, launches):
+    _lib.launches += launches
+    if rc != 0:
+        raise RuntimeError(f"{what}: {_lib.lib().rtp_flash_last_error().decode()}")
+
+
+def _window_fwd(q, k, v, window, sinks, sm_scale, want_lse):
+    if q.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(q.device):
+            return _window_fwd(q, k, v, window, sinks, sm_scale, want_lse)
+    B, Sq, H, _ = q.shape
+    q, k, v = _addressable(q), _addressable(k), _addressable(v)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(B * H, Sq, dtype=torch.float32, device=q.device) if want_lse else None
+    a = _window_args(q, k, v, o, lse, window, sinks, sm_scale)
+    _window_check(_lib.lib().rtp_window_fwd(C.byref(a), _lib.stream_ptr()), "rtp_window_fwd", 1)
+    return q, k, v, o, lse
+
+
+def _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale):
+    if q.device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(q.device):
+            return _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale)
+    do = _addressable(do)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    # blocks of keys that come before every window and hold no sink are not written
+    unseen = max(0, k.shape[1] - q.shape[1] - window + 1) // 128 > -(-min(sinks, k.shape[1]) // 128)
+    new = torch.zeros_like if unseen else torch.empty_like
+    dk, dv = (new(t, memory_format=torch.contiguous_format) for t in (k, v))
+    delta = torch.empty_like(lse)
+    a = _window_args(q, k, v, o, lse, window, sinks, sm_scale)
+    f = a.f
+    f.dout, f.dq, f.dk, f.dv, f.delta = _ref4(do), _ref4(dq), _shared_ref(dk, 1), _shared_ref(dv, 1), delta.data_ptr()
+    L = _lib.lib()
+    need = L.rtp_window_bwd_scratch(C.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.scratch, a.scratch_bytes = scratch.data_ptr(), need
+    _window_check(L.rtp_window_bwd(C.byref(a), _lib.stream_ptr()), "rtp_window_bwd", 3 if need else 2)
+    return dq, dk, dv
+
+
+class _WindowFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, sm_scale):
+        q, k, v, o, lse = _window_fwd(q, k, v, window, sinks, sm_scale, True)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.cfg = (window, sinks, sm_scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        return _window_bwd(*ctx.saved_tensors, do, *ctx.cfg) + (None,) * 3
+
+
+def window_attention(q, k, v, window, sinks=0, sm_scale=None):
+    """Kernel front-end of ``ops.functional.window_attention`` (same arguments): bf16 CUDA tensors, ``head_dim`` 64 or 128."""
+    check_window_args(q, k, v, window, sinks)
+    if not q.is_cuda or q.dtype != torch.bfloat16 or q.shape[3] not in (64, 128) or q.numel() == 0:
+        raise ValueError(f"window attention: the kernels take bf16 CUDA tensors with head_dim 64 or 128, got {q.dtype} {tuple(q.shape)} on {q.device}")
+    sm_scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowFn.apply(q, k, v, window, sinks, sm_scale)
+    return _window_fwd(q, k, v, window, sinks, sm_scale, False)[3]

@@ -179,6 +179,31 @@ def causal_attention(q, k, v):
     return o.transpose(1, 2)
 
 
+def window_attention(q, k, v, window, sinks=0, sm_scale=None):
+    """Causal attention over a sliding window with sinks: ``q`` [B, Sq, H, hd], ``k`` / ``v`` [B, Sk, Hk, hd] -> [B, Sq, H, hd] (views
+    are fine; ``H`` a multiple of ``Hk``, whose heads serve ``H / Hk`` neighbouring query heads each).
+
+    The queries are the last ``Sq <= Sk`` positions: query i stands at ``p = i + Sk - Sq`` and sees key j if ``j <= p`` and
+    (``j > p - window`` or ``j < sinks``).  ``sm_scale``: factor on the scores, ``hd ** -0.5`` by default.
+
+    bf16 CUDA tensors of head_dim 64 or 128 run on the tcgen05 kernels (``csrc/flash_attn.cu``): scores in fp32, probabilities and their
+    gradients rounded to bf16 for the products, sums in fp32."""
+    if use_kernels(q) and q.dim() == 4 and q.shape[3] in (64, 128) and q.numel():
+        from .flash import window_attention as run
+        return run(q, k, v, window, sinks, sm_scale)
+    from .flash import check_window_args
+    check_window_args(q, k, v, window, sinks)
+    B, Sq, H, hd = q.shape
+    Sk, Hk = k.shape[1:3]
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qq = q.to(acc).transpose(1, 2).reshape(B, Hk, (H // Hk) * Sq, hd)
+    s = (qq @ k.to(acc).permute(0, 2, 3, 1) * (hd ** -0.5 if sm_scale is None else sm_scale)).view(B, H, Sq, Sk)
+    p, j = torch.arange(Sk - Sq, Sk, device=q.device)[:, None], torch.arange(Sk, device=q.device)
+    s = s.masked_fill((j > p) | ((j <= p - window) & (j >= sinks)), float("-inf"))
+    o = s.softmax(-1).view(B, Hk, (H // Hk) * Sq, Sk) @ v.to(acc).transpose(1, 2)
+    return o.view(B, H, Sq, hd).transpose(1, 2).to(q.dtype)
+
+
 class _GeluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):

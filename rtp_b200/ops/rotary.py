@@ -105,9 +105,16 @@ def kernel_takes(q):
     return q.is_cuda and q.dtype in _TYPES and q.shape[3] <= 256 and q.shape[3] % 2 == 0
 
 
-def _strides(t):
-    """Strides of batch, position and head; those of a single one do not matter."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+def _side(t):
+    """(tensor, its output, addresses, strides) of q or k; strides of a single batch entry, position or head do not matter."""
+    if t is None:
+        return None, None, None, None, 0, 0, 0, 0
+    (B, S, H, _), (sb, ss, sh, sd) = t.shape, t.stride()
+    if sd != 1:
+        t = t.contiguous()
+        sb, ss, sh, _ = t.stride()
+    o = torch.empty_like(t, memory_format=torch.contiguous_format)
+    return t, o, t.data_ptr(), o.data_ptr(), sb if B > 1 else 0, ss if S > 1 else 0, sh if H > 1 else 0, H
 
 
 def _rotate(q, k, positions, freqs, half, magnitude, backward):
@@ -116,37 +123,19 @@ def _rotate(q, k, positions, freqs, half, magnitude, backward):
     if one.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(one.device):
             return _rotate(q, k, positions, freqs, half, magnitude, backward)
-    a = RotaryArgs()
-    a.B, a.S, _, a.hd = one.shape
-    outs = []
-    for side, t in (("q", q), ("k", k)):
-        if t is None:
-            outs.append(None)
-            continue
-        if t.stride(3) != 1:
-            t = t.contiguous()
-        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        outs.append(o)
-        setattr(a, side, t.data_ptr())
-        setattr(a, side + "o", o.data_ptr())
-        setattr(a, side + "_heads", t.shape[2])
-        for name, s in zip(("_sb", "_ss", "_sh"), _strides(t)):
-            setattr(a, side + name, s)
-        if side == "q":
-            q = t            # a copy lives until the launch
-        else:
-            k = t
+    B, S, _, hd = one.shape
+    q, qo, qp, qop, qb, qs, qh, H = _side(q)          # copies live until the launch
+    k, ko, kp, kop, kb, ks, kh, Hk = _side(k)
     freqs = freqs.contiguous()
-    a.positions, a.pos64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-    a.pos_ss = positions.stride(-1)
-    a.pos_sb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    a.freqs, a.rot = freqs.data_ptr(), 2 * freqs.shape[0]
-    a.magnitude, a.half_layout, a.dtype, a.backward = magnitude, int(half), _TYPES[one.dtype], int(backward)
+    st = positions.stride()
+    a = RotaryArgs(qp, kp, qop, kop, qb, qs, qh, kb, ks, kh, positions.data_ptr(), st[0] if len(st) == 2 and positions.shape[0] > 1 else 0,
+                   st[-1], freqs.data_ptr(), magnitude, positions.dtype == torch.int64, B, S, H, Hk, hd, 2 * freqs.shape[0], half,
+                   _TYPES[one.dtype], backward)
     L = _L()
     if L.rtp_rotary(C.byref(a), _lib.stream_ptr()) != 0:
         raise RuntimeError("rotary: " + L.rtp_rotary_last_error().decode())
     _lib.launches += 1
-    return outs
+    return qo, ko
 
 
 class _RotaryFn(torch.autograd.Function):
@@ -155,8 +144,7 @@ class _RotaryFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, freqs)
         ctx.cfg = (half, magnitude, backward)
-        qo, ko = _rotate(q, k, positions, freqs, half, magnitude, backward)
-        return qo, ko
+        return _rotate(q, k, positions, freqs, half, magnitude, backward)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -180,7 +168,7 @@ def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
     half, magnitude = layout == "half", float(magnitude)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, positions, freqs, half, magnitude, False)
-    return tuple(_rotate(q, k, positions, freqs, half, magnitude, False))
+    return _rotate(q, k, positions, freqs, half, magnitude, False)
 
 
 def rotary_plain(q, k, positions, freqs, layout="half", magnitude=1.0):
