@@ -85,6 +85,13 @@ struct MaskArgs {
   int window, sinks, ahead;
 };
 
+// n / d for n < 2^31 as a product: m = floor(2^(31 + s) / d) + 1 with 2^s >= d is off by a factor below 1 + 2^-31.  A window's pieces
+// of work are a few blocks long, and the divisions that look one up took 1 800 clocks of the 17 000 of a piece of three blocks.
+struct Div {
+  uint32_t m, s, d;
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((unsigned long long)(uint32_t)n * m) >> s); }
+};
+
 struct alignas(64) FlashParams {
   CUtensorMap mq, mk, mv, mdo;         // 3-D maps {columns, dim1, dim2}; *_seq1 tells which of dim1 / dim2 is the sequence
   int q_seq1, k_seq1, v_seq1, do_seq1;
@@ -94,6 +101,8 @@ struct alignas(64) FlashParams {
   int B, H;
   int group;                           // (batch, head) pairs whose CTAs run side by side (see head_group)
   int split;                           // forward: one row tile a CTA, its key blocks dealt to the two warpgroups
+  int pairs;                           // batch entries x key heads
+  Div by_heads, by_batch_heads, by_sink_work, by_sink_blocks, by_span, by_group, by_last_group, by_qpk, by_key_heads;
   // window: query heads that share a key head; key blocks that hold a sink; the first of the others that a query sees; pieces that the
   // queries of a block of sinks fall into, and where those leave their sums (null: one piece)
   int qpk, sink_blocks, first_block, pieces;
@@ -157,12 +166,9 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   }
 }
 
-// the bits below bit n (none for n <= 0, all for n >= 32)
-__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-
 // x[i] = log2-domain score of (row, col0 + i): scale, additive mask, key padding, causal and sequence bounds.
 // Masked entries become -inf.  `plain` = nothing but the scale applies to this block.  MSK: 0 no masks, 1 key padding only,
-// 2 an additive mask (with or without key padding), 3 window and sinks; `dead`: bit i set = key col0 + i is padding (dead_keys).
+// 2 an additive mask (with or without key padding); `dead`: bit i set = key col0 + i is padding (dead_keys).
 template <int NC, int MSK>
 __device__ __forceinline__ void score_chunk(float* x, int row, int col0, uint32_t dead, const MaskArgs& m, bool plain) {
   static_assert(NC == 32, "one word of bits");
@@ -203,13 +209,7 @@ __device__ __forceinline__ void score_chunk(float* x, int row, int col0, uint32_
   }
   // bit i: key col0 + i has no weight
   uint32_t off = MSK ? dead : 0u;
-  if constexpr (MSK == 3) {
-    const int pos = row + m.ahead;
-    off |= below(pos + 1 - col0) ^ 0xffffffffu;                                    // after the query
-    off |= below(pos + 1 - m.window - col0) & ~below(m.sinks - col0);              // before its window, no sink
-  } else {
   if (m.causal && col0 + NC - 1 > row) off |= row < col0 ? 0xffffffffu : 0xffffffffu << (row + 1 - col0);
-  }
   if (col0 + NC > m.Sk) off |= col0 >= m.Sk ? 0xffffffffu : 0xffffffffu << (m.Sk - col0);
   if (off) {
 #pragma unroll
@@ -296,10 +296,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // 2^x of two numbers that are not NaN on the multiply-add pipes, x >= -126 or taken as that: 2^round(x) rides in as an exponent, the
 // rest is a polynomial of degree 6 in [-1/2, 1/2] (least maximum relative error, by Remez exchange).  Relative error up to 1.1e-7
 // in fp32, not above ex2.approx; twice its instructions, but the special-function unit has only four lanes an SM quarter.
+// LOW = -127: everything up to -127, -inf too, becomes exactly 0 (the exponent field of 1 less 127, f = 0) and what lies between -127
+// and -126 less than 2^-126.
+template <int LOW = -126>
 __device__ __forceinline__ float2 ex2_poly2(float2 t) {
   const float2 magic = make_float2(12582912.f, 12582912.f);       // 1.5 * 2^23: rounds to integers, which stay in the low bits
-  t.x = fmaxf(t.x, -126.f);
-  t.y = fmaxf(t.y, -126.f);
+  t.x = fmaxf(t.x, (float)LOW);
+  t.y = fmaxf(t.y, (float)LOW);
   const float2 r = add2(t, magic);
   const float2 n = add2(r, make_float2(-12582912.f, -12582912.f));
   const float2 f = fma2(n, make_float2(-1.f, -1.f), t);
@@ -435,6 +438,19 @@ __device__ __forceinline__ Keys window_keys(const FlashParams& p, int tile) {
   k.n = k.ns + last_block(p.m, tile) - k.lo + 1;
   return k;
 }
+// the bits below bit n (none for n <= 0, all for n >= 32)
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// -infinity for those of 32 scores whose bit is not set.  Most chunks of a block that a border crosses lie on one side of it for a
+// whole warp.
+__device__ __forceinline__ void keep_seen(float* x, uint32_t seen) {
+  if (!__any_sync(0xffffffffu, seen != 0xffffffffu)) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = (seen >> i) & 1u ? x[i] : -INFINITY;
+}
+// bit i: the query at position `pos` sees key col0 + i
+__device__ __forceinline__ uint32_t keys_seen(const MaskArgs& m, int pos, int col0) {
+  return below(pos + 1 - col0) & (~below(pos + 1 - m.window - col0) | below(m.sinks - col0));
+}
 // Whether every query of the 128 from q0 on sees all of the 128 keys from k0 on.
 __device__ __forceinline__ bool all_seen(const MaskArgs& m, int q0, int k0) {
   return k0 + kBlk - 1 <= q0 + m.ahead && (k0 > q0 + kBlk - 1 + m.ahead - m.window || k0 + kBlk <= m.sinks);
@@ -461,8 +477,26 @@ struct FwdWork {
   int s1;                              // window: the second tile's first step
   Keys keys;
 };
+// Window: last row tiles first, the heads of a tile side by side.
+__device__ __forceinline__ FwdWork window_fwd_work(const FlashParams& p, int blk) {
+  const int nqb = (p.m.Sq + kBlk - 1) / kBlk, level = p.by_batch_heads(blk);
+  FwdWork w;
+  w.bh = blk - level * (int)p.by_batch_heads.d;
+  w.b = p.by_heads(w.bh);
+  w.h = w.bh - w.b * p.H;
+  w.g0 = p.split ? nqb - 1 - level : (((nqb + 1) >> 1) - 1 - level) * 2;
+  w.keys = window_keys(p, w.g0);
+  const int nb0 = w.keys.n;
+  const bool two = !p.split && w.g0 + 1 < nqb;
+  w.n0 = p.split ? (nb0 + 1) >> 1 : nb0;
+  w.n1 = p.split ? nb0 >> 1 : two ? nb0 + last_block(p.m, w.g0 + 1) - last_block(p.m, w.g0) : 0;
+  w.s1 = two && (w.keys.lo > 0 || p.sink_blocks == 0) ? window_block(p.m, w.g0 + 1) - w.keys.lo : 0;
+  w.nload = p.split ? nb0 : max(w.n0, w.n1);
+  return w;
+}
 template <bool WIN>
 __device__ __forceinline__ FwdWork fwd_work(const FlashParams& p, int blk) {
+  if constexpr (WIN) return window_fwd_work(p, blk);
   const int nqb = (p.m.Sq + kBlk - 1) / kBlk, nkb = (p.m.Sk + kBlk - 1) / kBlk, BH = p.B * p.H;
   // row tiles of a piece of work: one or two; heaviest (last) query blocks of a group of heads first
   const int nt = p.split ? nqb : (nqb + 1) >> 1, span = p.group * nt;
@@ -474,21 +508,11 @@ __device__ __forceinline__ FwdWork fwd_work(const FlashParams& p, int blk) {
   }
   const int heads = min(p.group, BH - grp), level = blk / heads;
   FwdWork w;
+  w.s1 = 0;
   w.g0 = (nt - 1 - level) * (p.split ? 1 : 2);
   w.bh = grp + blk - level * heads;
   w.b = w.bh / p.H;
   w.h = w.bh - w.b * p.H;
-  w.s1 = 0;
-  if constexpr (WIN) {
-    w.keys = window_keys(p, w.g0);
-    const int nb0 = w.keys.n;
-    const bool two = !p.split && w.g0 + 1 < nqb;
-    w.n0 = p.split ? (nb0 + 1) >> 1 : nb0;
-    w.n1 = p.split ? nb0 >> 1 : two ? nb0 + last_block(p.m, w.g0 + 1) - last_block(p.m, w.g0) : 0;
-    if (two && (w.keys.lo > 0 || p.sink_blocks == 0)) w.s1 = window_block(p.m, w.g0 + 1) - w.keys.lo;
-    w.nload = p.split ? nb0 : max(w.n0, w.n1);
-    return w;
-  }
   const int nb0 = p.m.causal ? min(nkb, w.g0 + 1) : nkb;            // key blocks of the first tile, of the second
   const int nb1 = w.g0 + 1 >= nqb ? 0 : p.m.causal ? min(nkb, w.g0 + 2) : nkb;
   w.n0 = p.split ? (nb0 + 1) >> 1 : nb0;
@@ -671,7 +695,8 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       // for all blocks; one that only needs the scale keeps the raw scores: the scale rides in the exponent's multiply-add.
       const bool unmasked = WIN ? all_seen(M, gt * kBlk, col0)
                                 : MSK != 2 && !(dead[0] | dead[1] | dead[2] | dead[3]) && !(M.causal && c == gt);
-      const bool plain = unmasked && (col0 + kBlk <= M.Sk) && M.scale_log2 >= 0.f;   // the maximum commutes with a positive scale only
+      // the maximum commutes with a positive scale only (which a window's is)
+      const bool plain = WIN || (unmasked && (col0 + kBlk <= M.Sk) && M.scale_log2 >= 0.f);
       if (!plain) {
         constexpr int NQ = MSK == 2 ? 1 : 2;           // chunks at a time: the additive mask's code is long
 #pragma unroll 1
@@ -683,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
 #pragma unroll
           for (int u = 0; u < NQ; ++u) {
             const uint32_t dd = q + u == 0 ? dead[0] : q + u == 1 ? dead[1] : q + u == 2 ? dead[2] : dead[3];
-            score_chunk<32, MSK>(x + 32 * u, row, col0 + 32 * (q + u), dd, M, false);
+            score_chunk<32, MSK == 3 ? 0 : MSK>(x + 32 * u, row, col0 + 32 * (q + u), dd, M, false);
             tmem_st32f(aS + (uint32_t)((q + u) * 32), x + 32 * u);
           }
         }
@@ -695,8 +720,16 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       tmem_ld_wait();
       tmem_ld32f(aS + 64, s + 64);
       tmem_ld32f(aS + 96, s + 96);
+      if (WIN && !unmasked) {
+        keep_seen(s, keys_seen(M, row + M.ahead, col0));
+        keep_seen(s + 32, keys_seen(M, row + M.ahead, col0 + 32));
+      }
       float mx = max64(s);
       tmem_ld_wait();
+      if (WIN && !unmasked) {
+        keep_seen(s + 64, keys_seen(M, row + M.ahead, col0 + 64));
+        keep_seen(s + 96, keys_seen(M, row + M.ahead, col0 + 96));
+      }
       mx = max3(mx, mx, max64(s + 64));
       if (plain) mx *= M.scale_log2;
       const float cand = fmaxf(m_used, mx);
@@ -707,7 +740,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       // some: one exponential in four by polynomial.  That is for blocks without masked scores, which have to become 0, whose rows
       // all have a finite maximum: a NaN or an infinite score has to reach the output, and a row of -inf alone has no weights;
       // a -inf below a finite maximum gets 2^-126 beside 2^-8 or more.
-      const bool fin = fabsf(mx) < INFINITY;
+      // Window: hidden scores, -inf, become exactly 0 by either way, so all blocks take the one: the other's code beside it cost
+      // more in instruction fetch than its exponentials.
+      const bool fin = WIN ? mx < INFINITY : fabsf(mx) < INFINITY;
       bool some = !DRP && plain;
       if (__any_sync(0xffffffffu, (i > begin && need) || !fin)) {
         if (i > begin && __any_sync(0xffffffffu, need)) {
@@ -739,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
         for (int k = 0; k < 32; k += 4) {
           float2 x = fma2(make_float2(e[k], e[k + 1]), mul2, ref2), y = fma2(make_float2(e[k + 2], e[k + 3]), mul2, ref2);
           x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-          if (decltype(poly)::value && (k & 4)) y = ex2_poly2(y);
+          if (decltype(poly)::value && (k & 4)) y = ex2_poly2<WIN ? -127 : -126>(y);
           else y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
           ra = add2(ra, x);
           rb = add2(rb, y);
@@ -898,42 +933,45 @@ struct BwdWork {
 // blocks and behind them, as they are `qpk` times as short, the query blocks of its heads.
 __device__ __forceinline__ BwdWork window_work(const FlashParams& p, int blk) {
   const MaskArgs& m = p.m;
-  const int nq = (m.Sq + kBlk - 1) / kBlk, nk = (m.Sk + kBlk - 1) / kBlk, heads_k = p.H / p.qpk, BK = p.B * heads_k;
+  const int nq = (m.Sq + kBlk - 1) / kBlk, nk = (m.Sk + kBlk - 1) / kBlk;
   BwdWork w = {-1, -1, 0, 0, 0, 0, 0, 0, 0, -1, {0, 0, 0}};
-  int pair, of = 0, pieces = 1;                             // pair: (batch, key head)
-  const int sink_work = BK * p.sink_blocks * p.pieces;
+  int pair, of = 0;                                         // pair: (batch, key head)
+  const int sink_work = (int)p.by_sink_work.d * p.pieces;   // by_sink_work.d: pairs x blocks of sinks
   if (blk < sink_work) {
-    of = blk / (BK * p.sink_blocks);
-    blk -= of * BK * p.sink_blocks;
-    pair = blk / p.sink_blocks;
+    of = p.by_sink_work(blk);
+    blk -= of * (int)p.by_sink_work.d;
+    pair = p.by_sink_blocks(blk);
     w.kb = blk - pair * p.sink_blocks;
-    pieces = p.pieces;
-    if (p.part) w.piece = (pair * p.sink_blocks + w.kb) * pieces + of;
+    if (p.part) w.piece = (pair * p.sink_blocks + w.kb) * p.pieces + of;
   } else {
     blk -= sink_work;
-    const int nkb = nk - p.first_block, per = nkb + nq * p.qpk, span = p.group * per;
-    const int g = blk / span, grp = g * p.group, heads = min(p.group, BK - grp);
-    blk -= g * span;
-    const int row = blk / heads;
-    pair = grp + blk - row * heads;
+    const int g = p.by_span(blk), grp = g * p.group;
+    blk -= g * (int)p.by_span.d;
+    const bool last = grp + p.group > p.pairs;
+    const Div& by = last ? p.by_last_group : p.by_group;
+    const int row = by(blk), nkb = nk - p.first_block;
+    pair = grp + blk - row * (int)by.d;
     if (row < nkb) w.kb = p.first_block + row;
     else {
-      const int r = row - nkb;
-      w.qb = nq - 1 - r / p.qpk;
-      w.h = r % p.qpk;
+      const int r = row - nkb, q = p.by_qpk(r);
+      w.qb = nq - 1 - q;
+      w.h = r - q * p.qpk;
     }
   }
-  w.b = pair / heads_k;
-  w.h += (pair - w.b * heads_k) * p.qpk;
+  w.b = p.by_key_heads(pair);
+  w.h += (pair - w.b * (int)p.by_key_heads.d) * p.qpk;
   w.bh = w.b * p.H + w.h;
   if (w.kb >= 0) {
     w.q0 = max(0, w.kb * kBlk - m.ahead) / kBlk;
     // the last query that sees the block's last key; a sink is seen to the end
     const long long last = (long long)w.kb * kBlk + kBlk - 2 + m.window - m.ahead;
     w.nq = (w.kb < p.sink_blocks ? nq : (int)min((long long)nq, last / kBlk + 1)) - w.q0;
-    const int all = w.nq * p.qpk;
-    w.s0 = (int)((long long)all * of / pieces);
-    w.n = (int)((long long)all * (of + 1) / pieces) - w.s0;
+    w.n = w.nq * p.qpk;
+    if (w.piece >= 0) {
+      const long long all = w.n;
+      w.s0 = (int)(all * of / p.pieces);
+      w.n = (int)(all * (of + 1) / p.pieces) - w.s0;
+    }
   } else {
     w.keys = window_keys(p, w.qb);
     w.n = w.keys.n;
@@ -1019,8 +1057,13 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
       if (w.kb >= 0) {
         const int i0 = WIN ? w.s0 : M.causal ? w.kb : 0, i1 = WIN ? w.s0 + w.n : nqb;
         ok = load(0, &p.mk, p.k_seq1, ck, b, w.kb * kBlk);
+        int hq = 0, off = 0;                            // window: head and query block of the step
+        if (WIN && w.s0) {
+          hq = w.s0 / w.nq;
+          off = w.s0 - hq * w.nq;
+        }
         for (int i = i0; i < i1 && ok; ++i) {
-          const int st = (i - i0) & 1, hq = WIN ? i / w.nq : 0, q0 = (WIN ? w.q0 + i - hq * w.nq : i) * kBlk;
+          const int st = (i - i0) & 1, q0 = (WIN ? w.q0 + off : i) * kBlk;
           const long long base = (long long)(w.bh + hq) * M.Sq;
           ok = load(2 + st, &p.mq, p.q_seq1, WIN ? head_col(p.q, h + hq) : cq, b, q0);
           if (!ok) break;
@@ -1034,6 +1077,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
             stat[kBlk + e * 32 + lane] = q < M.Sq ? -__ldg(p.delta + base + q) : 0.f;
           }
           mbar_arrive(&bar[B_STAT + st]);
+          if (WIN && ++off == w.nq) { off = 0; ++hq; }
         }
       } else {
         const int nb = WIN ? w.n : M.causal ? min(nkb, w.qb + 1) : nkb;
@@ -1151,9 +1195,11 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
         bool key_dead = key >= M.Sk;
         if constexpr (MSK == 1 || MSK == 2) key_dead = key_dead || (M.kpm && __ldg(M.kpm + (long long)b * M.kpm_ld + key));
         const bool keys_plain = MSK != 2 && !__any_sync(0xffffffffu, key_dead);
+        int qoff = WIN && w.s0 ? w.s0 % w.nq : 0;
         for (int it = 0; it < nit; ++it) {
           const int st = it & 1;
-          const int qb = WIN ? w.q0 + (i0 + it) % w.nq : i0 + it;
+          const int qb = WIN ? w.q0 + qoff : i0 + it;
+          if (WIN && ++qoff == w.nq) qoff = 0;
           const int qbase = qb * kBlk + wg * 64;                 // first query of this thread
           const float* nlse = sStat + st * 2 * kBlk + wg * 64;
           const float* ndel = nlse + kBlk;
@@ -1196,6 +1242,16 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
               const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, make_float2(nl[i], nl[i + 1]));
               x[i] = u.x; x[i + 1] = u.y;
             }
+          } else if constexpr (WIN) {
+            // the queries that see the key: from its own position to the end of the window, a sink to the last
+            const int lo = key - M.ahead - qbase, hi = key_dead ? lo : key < M.sinks ? 64 : lo + M.window;
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, make_float2(nl[i], nl[i + 1]));
+              x[i] = u.x; x[i + 1] = u.y;
+            }
+            keep_seen(x, below(hi) & ~below(lo));
+            keep_seen(x + 32, below(hi - 32) & ~below(lo - 32));
           } else {
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
@@ -1208,9 +1264,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
                                      : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(M.mask) + mi))) * kLog2e;
                 }
               }
-              bool hidden = M.causal && key > q;
-              if constexpr (WIN) hidden = key > q + M.ahead || (key <= q + M.ahead - M.window && key >= M.sinks);
-              x[i] = key_dead || hidden ? -INFINITY : xs + nl[i];
+              x[i] = key_dead || (M.causal && key > q) ? -INFINITY : xs + nl[i];
             }
           }
 #pragma unroll
@@ -1287,16 +1341,20 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           tmem_ld32f(aS + 32, x + 32);
           tmem_ld_wait();
           const bool unmasked = WIN ? all_seen(M, q0, kb * kBlk) : MSK != 2 && !(dead[0] | dead[1]) && !(M.causal && j == w.qb);
-          const bool plain = unmasked && (kb * kBlk + kBlk <= M.Sk);
+          const bool plain = WIN || (unmasked && (kb * kBlk + kBlk <= M.Sk));
           if (plain) {
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
               const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, nl);
               x[i] = u.x; x[i + 1] = u.y;
             }
+            if (WIN && !unmasked) {
+              keep_seen(x, keys_seen(M, row + M.ahead, col0));
+              keep_seen(x + 32, keys_seen(M, row + M.ahead, col0 + 32));
+            }
           } else {
-            score_chunk<32, MSK>(x, row, col0, dead[0], M, false);
-            score_chunk<32, MSK>(x + 32, row, col0 + 32, dead[1], M, false);
+            score_chunk<32, MSK == 3 ? 0 : MSK>(x, row, col0, dead[0], M, false);
+            score_chunk<32, MSK == 3 ? 0 : MSK>(x + 32, row, col0 + 32, dead[1], M, false);
 #pragma unroll
             for (int i = 0; i < 64; ++i) x[i] += nlse;
           }
@@ -1329,11 +1387,46 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
       tc_fence_after();
       const int r0 = (w.kb >= 0 ? w.kb : w.qb) * kBlk + (warp & 3) * 32;      // the warp's first row
       const int nacc = ONE ? 3 : w.kb >= 0 ? 2 : 1;
+      if constexpr (WIN) {               // everything at once: one wait, and the accumulators are free for the next piece
+        float o[HD];                     // dV and dK, half a row each, or that of dQ
+        const bool is_q = w.kb < 0;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int c = 0; c < HD / 64; ++c)
+            if (a == 0 || !is_q) tmem_ld32f(tAcc + (uint32_t)(a * HD) + lane_off + (uint32_t)(wg * (HD / 2) + c * 32), o + a * (HD / 2) + c * 32);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar[B_ACCREAD]);
+        const float mul0 = is_q ? M.sm_scale : 1.f;
+#pragma unroll
+        for (int i = 0; i < HD / 2; ++i) { o[i] *= mul0; o[HD / 2 + i] *= M.sm_scale; }
+        if (w.piece >= 0) {              // [piece][dV, dK][HD / 4][key][4]: the lanes of a store side by side
+          float4* sum = reinterpret_cast<float4*>(p.part) + (long long)w.piece * 2 * (HD / 4) * kBlk + wg * (HD / 8) * kBlk + rt;
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+              const float* e = o + a * (HD / 2) + 4 * i;
+              sum[(a * (HD / 4) + i) * kBlk] = make_float4(e[0], e[1], e[2], e[3]);
+            }
+        } else {
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            if (a && is_q) break;
+            const DRef& out = is_q ? p.dq : a ? p.dk : p.dv;
+            __nv_bfloat16* dst = row_ptr(out, b, r0, is_q ? h : p.by_qpk(h)) + wg * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) store_rows32(dst + c * 32, out.ss, (is_q ? M.Sq : M.Sk) - r0, o + a * (HD / 2) + c * 32, lane);
+          }
+        }
+      } else
       for (int a = 0; a < nacc; ++a) {
         const bool is_q = w.kb < 0 || (ONE && a == 2);
         const DRef& out = is_q ? p.dq : a ? p.dk : p.dv;
         const int left = (is_q ? M.Sq : M.Sk) - r0;
-        __nv_bfloat16* dst = row_ptr(out, b, r0, WIN && !is_q ? h / p.qpk : h) + wg * (HD / 2);
+        __nv_bfloat16* dst = row_ptr(out, b, r0, h) + wg * (HD / 2);
         const float mul = !is_q && a == 0 ? 1.f : M.sm_scale;
         const uint32_t acc = ONE && a == 2 ? tS : tAcc + (uint32_t)(a * HD);
 #pragma unroll
@@ -1348,13 +1441,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] *= mul;
-          if (WIN && w.piece >= 0) {     // [piece][dV, dK][HD / 4][key][4]: the lanes of a store side by side
-            float4* sum = reinterpret_cast<float4*>(p.part) + ((long long)w.piece * 2 + a) * (HD / 4) * kBlk + (wg * (HD / 8) + c * 8) * kBlk + rt;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i * kBlk] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          } else {
-            store_rows32(dst + c * 32, out.ss, left, o, lane);
-          }
+          store_rows32(dst + c * 32, out.ss, left, o, lane);
         }
       }
     }
@@ -1538,12 +1625,20 @@ int fill_common(const RtpFlashArgs* a, FlashParams& P) {
   P.q = dref(a->q); P.k = dref(a->k); P.v = dref(a->v); P.o = dref(a->o);
   return 0;
 }
+Div divider(int d) {
+  Div r = {0, 31, (uint32_t)d};
+  if (d < 1) return r;                 // never asked
+  while ((1ll << (r.s - 31)) < d) ++r.s;
+  r.m = (uint32_t)((1ull << r.s) / (unsigned)d + 1);
+  return r;
+}
 // What the window kernels need beside the common part.
 int fill_window(const RtpWindowArgs* w, FlashParams& P) {
   const RtpFlashArgs& a = w->f;
   if (a.causal || a.mask || a.kpm || a.drop_p != 0.f) return ffail("window attention: no other mask and no dropout");
   if (w->kv_heads <= 0 || a.H % w->kv_heads) return ffail("window attention: the query heads must be a multiple of the key heads");
   if (a.Sq > a.Sk) return ffail("window attention: more queries than keys");
+  if (!(a.sm_scale > 1e-30f && a.sm_scale < 1e30f)) return ffail("window attention: the scale must be positive");
   if (w->window < 1 || w->sinks < 0) return ffail("window attention: a window of at least one key, no negative number of sinks");
   if (fill_common(&a, P)) return -1;
   P.m.window = std::min(w->window, a.Sk);
@@ -1554,6 +1649,10 @@ int fill_window(const RtpWindowArgs* w, FlashParams& P) {
   P.first_block = std::max(P.sink_blocks, std::max(0, P.m.ahead - P.m.window + 1) / kBlk);
   P.pieces = 1;
   P.part = nullptr;
+  P.pairs = a.B * w->kv_heads;
+  P.by_heads = divider(a.H);
+  P.by_qpk = divider(P.qpk);
+  P.by_key_heads = divider(w->kv_heads);
   return 0;
 }
 // Pieces that the queries of a block of sinks fall into.  All queries see a sink: over a long context its block would be many times
@@ -1623,12 +1722,13 @@ int rtp_window_fwd(const RtpWindowArgs* w, void* stream) {
   static thread_local FlashParams P;
   if (fill_window(w, P)) return -1;
   const RtpFlashArgs* a = &w->f;
+  if ((long long)a->B * a->H > 0x7fffffffll) return ffail("window attention: problem too large");
   const int tiles = (a->Sq + kBlk - 1) / kBlk, BH = a->B * a->H;
   P.split = (long long)tiles * BH <= device_sms();              // as without a window
-  // whole groups of heads that share their keys
-  const int g = head_group(4ll * std::min(a->Sk, P.m.window + 2 * kBlk) * a->head_dim, BH);
-  P.group = std::min(BH, std::max(P.qpk, g / P.qpk * P.qpk));
-  const int grid = (P.split ? tiles : (tiles + 1) / 2) * BH;
+  P.by_batch_heads = divider(BH);
+  const long long total = (long long)(P.split ? tiles : (tiles + 1) / 2) * BH;
+  if (total > 0x7fffffffll) return ffail("window attention: problem too large");
+  const int grid = (int)total;
   return launched((a->head_dim == 64 ? rtp_flash_part_fwd64 : rtp_flash_part_fwd128)(&P, 3, 0, grid > device_sms(), grid, stream),
                   "window_fwd");
 }
@@ -1658,15 +1758,22 @@ int rtp_window_bwd(const RtpWindowArgs* w, void* stream) {
     P.pieces = sink_pieces(w, device_sms());
   }
   const int nq = (a->Sq + kBlk - 1) / kBlk, nk = (a->Sk + kBlk - 1) / kBlk, BK = a->B * w->kv_heads;
-  const long long grid = (long long)BK * (P.sink_blocks * P.pieces + nk - P.first_block + (long long)nq * P.qpk);
-  if (grid > 0x7fffffffll) return ffail("window attention backward: problem too large");
+  const long long total = (long long)BK * (P.sink_blocks * P.pieces + nk - P.first_block + (long long)nq * P.qpk);
+  if (total > 0x7fffffffll) return ffail("window attention backward: problem too large");
+  const int grid = (int)total;
   P.group = head_group(4ll * (std::min(a->Sq, P.m.window) * (long long)P.qpk + std::min(a->Sk, P.m.window)) * a->head_dim, BK);
+  const int per = nk - P.first_block + nq * P.qpk;
+  P.by_sink_work = divider(BK * P.sink_blocks);
+  P.by_sink_blocks = divider(P.sink_blocks);
+  P.by_span = divider(P.group * per);
+  P.by_group = divider(P.group);
+  P.by_last_group = divider(BK % P.group ? BK % P.group : P.group);
   cudaStream_t s = (cudaStream_t)stream;
-  const long long rows = (long long)a->B * a->Sq * a->H, per = 256 / (a->head_dim / 8);
+  const long long rows = (long long)a->B * a->Sq * a->H, lanes = 256 / (a->head_dim / 8);
   cudaError_t e = launch_k(a->head_dim == 64 ? flash_delta_kernel<64> : flash_delta_kernel<128>,
-                           dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
+                           dim3((unsigned)((rows + lanes - 1) / lanes)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
   if (e != cudaSuccess) return ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
-  if (launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, 3, 0, grid > 2 * device_sms(), (int)grid, stream),
+  if (launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, 3, 0, grid > 2 * device_sms(), grid, stream),
                "window_bwd"))
     return -1;
   if (!P.part) return 0;

@@ -340,6 +340,8 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     if not q.is_cuda or q.dtype != torch.bfloat16 or q.shape[3] not in (64, 128) or q.numel() == 0:
         raise ValueError(f"window attention: the kernels take bf16 CUDA tensors with head_dim 64 or 128, got {q.dtype} {tuple(q.shape)} on {q.device}")
     sm_scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 1e-30 < sm_scale < 1e30:
+        raise ValueError(f"window attention: the kernels take a positive sm_scale, got {sm_scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowFn.apply(q, k, v, window, sinks, sm_scale)
     return _window_fwd(q, k, v, window, sinks, sm_scale, False)[3]

@@ -102,7 +102,7 @@ def test_pieces_of_sinks_are_taken():
     assert _lib.lib().rtp_window_bwd_scratch(C.byref(a)) > 0
 
 
-@pytest.mark.parametrize("scale", [-0.3, 1.0, 1e-3])
+@pytest.mark.parametrize("scale", [0.3, 1.0, 1e-3])
 def test_scales(scale):
     check(*tensors(2, 300, 300, 4, 2, 64), 100, 3, scale)
 
@@ -222,6 +222,9 @@ def test_refusals_on_the_gpu():
     for bad in ((q.float(), k.float(), v.float()), (q[..., :32], k[..., :32], v[..., :32]), (q[:0], k[:0], v[:0])):
         with pytest.raises(ValueError):
             flash.window_attention(*bad, 4)
+    for scale in (0.0, -0.5, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            FO.window_attention(q, k, v, 4, sm_scale=scale)
     # those run in PyTorch operations behind the public entry point
     assert FO.window_attention(q.float(), k.float(), v.float(), 4).dtype == torch.float32
     assert FO.window_attention(q[..., :32], k[..., :32], v[..., :32], 4).shape == (1, 10, 2, 32)
