@@ -28,6 +28,38 @@ typedef struct {
 } RtpGemmArgs;
 int rtp_gemm(const RtpGemmArgs* args, void* stream);
 
+// Gated feed-forward block y = (silu(x Wg^T) * (x Wu^T)) Wd^T on this GPU alone: x [T, D], w_gu [2 F, D] (the rows of Wg before those of
+// Wu), w_d [O, F]; D, F and O multiples of 8, rows 16-byte aligned, everything bf16 with fp32 sums; gate, up, their product h and their
+// gradients are rounded to bf16.  gu, dgu [T, 2 F], h [T, F], y [T, O], dx [T, D], dw_gu and dw_d are dense.
+typedef struct {
+  int T, D, F, O;
+  const void* x; long long ldx;
+  const void* w_gu; long long ld_gu;
+  const void* w_d; long long ld_d;
+  void* gu;                                   // the two projections, for the backward (null: not kept)
+  void* h;                                    // workspace
+  void* y;
+  unsigned long long* status;
+  void* scratch; unsigned long long scratch_bytes;   // rtp_gated_fwd_scratch() bytes, 16-byte aligned (none: null)
+} RtpGatedFwd;
+int rtp_gated_fwd(const RtpGatedFwd* args, void* stream);                 // two launches, three with scratch
+unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* args);
+typedef struct {
+  int T, D, F, O;
+  const void* x; long long ldx;
+  const void* dy; long long ldy;
+  const void* w_gu; long long ld_gu;
+  const void* w_d; long long ld_d;
+  const void* gu;                             // as the forward left it
+  void* dgu;                                  // workspace
+  void* h;                                    // workspace, needed for dw_d
+  void *dx, *dw_gu, *dw_d;                    // each may be null
+  unsigned long long* status;
+  void* scratch; unsigned long long scratch_bytes;
+} RtpGatedBwd;
+int rtp_gated_bwd(const RtpGatedBwd* args, void* stream);
+unsigned long long rtp_gated_bwd_scratch(const RtpGatedBwd* args);
+
 // Batched GEMM over windows of two 2-D tensors: batch z = (zo, zi), zi = z % batch_inner.  Operand X (stored
 // [x_rows, x_cols] row-major, pitch ldx) is read at row/column offsets zo * x_bo_* + zi * x_bi_* (in the operand's
 // own (mn, k) coordinates); the output moves by zo * d_bo + zi * d_bi elements.  Used for attention, where the

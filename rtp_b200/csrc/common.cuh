@@ -444,6 +444,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
+// silu(g) * u, and its gradients for the incoming d
+__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+__device__ __forceinline__ void swiglu_grad(float g, float u, float d, float& dg, float& du) {
+  const float sg = 1.f / (1.f + __expf(-g));
+  const float silu = g * sg;
+  du = d * silu;
+  dg = d * u * (sg + silu * (1.f - sg));
+}
+
 // A maximum that keeps a NaN, as fmaxf does not.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;

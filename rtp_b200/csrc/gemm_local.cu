@@ -71,6 +71,10 @@ struct alignas(64) Params {
   int ones_off;                                  // where the tile of ones starts behind the stage ring; 0: no sums
   unsigned long long* status;
   unsigned long long timeout_ns;
+  // gated feed-forward (see LocalGemm::gate); gate_cols: F
+  __nv_bfloat16 *gu, *dgu;
+  long long ldgu, lddgu;
+  int gate_cols;
   Job job[MAXJ];
 };
 
@@ -133,7 +137,14 @@ __device__ __forceinline__ int tile_kblocks(const Job& J, int s, int row0) {
 // launch: twice the spills, and a fifth of the epilogue's time went into instruction fetch.  With it compiled out and both
 // halves of a row's 64 columns fetched at once (us, before -> now): 256 x 64 -> 256 4.5 -> 3.4, 1024 x 512 -> 512 6.6 -> 5.5,
 // 1024 x 2048 -> 2048 13.4 -> 12.4, 8192 x 8 -> 8192 73 -> 45, 36864 x 64 -> 288 20 -> 13.6; added to its output 25 -> 21.
-template <bool PAIR, int MAXJ, bool SRC, bool FUN, bool FILL>
+// GATE 1: the first half of a tile's columns are the gate's, the second half the up projection's columns of the same place (on a pair
+// each CTA stages the rows of one of them), so a row's two numbers meet in one thread and gate, up and their product leave together:
+// [2 F, K] weights of two halves that a GEMM of its own would write and a pass of its own read back.
+// GATE 2: the epilogue turns the gradient of the product into those of gate and up, which it reads, and makes the product again for the
+// weight gradient behind it.
+// Both round what they hand on to bf16 as the separate launches did (the stored gate and up are what the product is made of), so the
+// fused block gives their bits.
+template <bool PAIR, int MAXJ, bool SRC, bool FUN, bool FILL, int GATE>
 __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_constant__ Params<MAXJ> P) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -221,7 +232,14 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
             tma_load_2d_s(sa, ma, m0, k0, bar);
             tma_load_2d_s(sa + 8192, ma, m0 + 64, k0, bar);
           } else tma_load_2d_s(sa, ma, k0, m0, bar);
-          if (sum) {
+          if constexpr (GATE == 1) {
+            const int row = tn * (J.bn >> 1);              // of the gate; the up projection's is gate_cols further
+            if (PAIR) tma_load_2d_s(sb, mb, k0, row + (int)crank * P.gate_cols, bar);
+            else {
+              tma_load_2d_s(sb, mb, k0, row, bar);
+              tma_load_2d_s(sb + (J.bn >> 1) * (kKB * 2), mb, k0, row + P.gate_cols, bar);
+            }
+          } else if (sum) {
           } else if (b3) tma_load_3d_s(sb, mb, 0, k0, n0 >> 6, bar);
           else if (b_mn) {
             for (int i = 0; i < nb; ++i) tma_load_2d_s(sb + i * 8192, mb, n0 + i * 64, k0, bar);
@@ -385,7 +403,52 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
           else d[m] = __float2bfloat16(__uint_as_float(ra[0]) + (c ? __bfloat162float(c[m]) : 0.f));
         }
       }
-      for (int ch = half; !J.sum && ch * 64 < bn; ch += 2) {
+      if constexpr (GATE == 1) {
+        uint32_t good = 1;
+        if (lane == 0) good = mbar_wait(&ctl->tmem_full[acc], acc_phase, abort_flag, status, tmo) ? 1u : 0u;
+        good = __shfl_sync(0xffffffffu, good, 0);
+        if (!good) { ok = false; break; }
+        tc_fence_after();
+        waited = true;
+        // 32 columns of both at a time: two staged rows of 64 bytes a thread, 16-byte chunk q at q ^ (row / 2) % 4
+        const int cols = bn >> 1, per = cols >> 6;         // columns of a tile, pieces of a warp
+        uint8_t* mine = stg + lane * 64;
+        const int sw = (lane >> 1) & 3;
+        for (int pc = half * per; pc < (half + 1) * per; ++pc) {
+          uint32_t ra[2][32];
+          const uint32_t acc_addr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * 256 + pc * 32);
+          tmem_ld_32x32(acc_addr, ra[0]);
+          tmem_ld_32x32(acc_addr + (uint32_t)cols, ra[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = pack_bf16(__uint_as_float(ra[t][8 * q + 2 * i]), __uint_as_float(ra[t][8 * q + 2 * i + 1]));
+              *reinterpret_cast<uint4*>(mine + t * 2048 + ((q ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          __syncwarp();
+          const int col = tn * cols + pc * 32 + (lane & 3) * 8;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = 8 * k + (lane >> 2), row = row0 + r;
+            const uint8_t* at = stg + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4);
+            const uint4 g = *reinterpret_cast<const uint4*>(at), u = *reinterpret_cast<const uint4*>(at + 2048);
+            if (row >= M || col >= P.gate_cols) continue;
+            if (P.gu) {
+              __nv_bfloat16* to = P.gu + (long long)row * P.ldgu + col;
+              *reinterpret_cast<uint4*>(to) = g;
+              *reinterpret_cast<uint4*>(to + P.gate_cols) = u;
+            }
+            auto two = [](uint32_t a, uint32_t b) { return pack_bf16(swiglu(bf16_lo(a), bf16_lo(b)), swiglu(bf16_hi(a), bf16_hi(b))); };
+            *reinterpret_cast<uint4*>(d + (long long)row * ldd + col) = make_uint4(two(g.x, u.x), two(g.y, u.y), two(g.z, u.z), two(g.w, u.w));
+          }
+          __syncwarp();
+        }
+      }
+      for (int ch = half; GATE != 1 && !J.sum && ch * 64 < bn; ch += 2) {
         const int col0 = n0 + ch * 64;
         const int ccol = col0 + (lane & 7) * 8;                      // column of this lane in the coalesced view
         // the accumulate source is fetched while the accumulator is still being made
@@ -402,12 +465,23 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
             }
           }
         }
+        [[maybe_unused]] uint4 gv[8], uv[8];             // gate and up, fetched likewise
+        if constexpr (GATE == 2) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = row0 + 4 * k + (lane >> 3);
+            const bool in = row < M && ccol < N;
+            const __nv_bfloat16* from = P.gu + (long long)row * P.ldgu + ccol;
+            gv[k] = in ? __ldcg(reinterpret_cast<const uint4*>(from)) : make_uint4(0u, 0u, 0u, 0u);
+            uv[k] = in ? __ldcg(reinterpret_cast<const uint4*>(from + P.gate_cols)) : make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
         // so is the bias, where no other source takes the registers (a job with both is rare)
         [[maybe_unused]] uint4 bv[8];
         auto bias8 = [&](int q) {
           return bias && col0 + q * 8 < N ? __ldg(reinterpret_cast<const uint4*>(bias + col0 + q * 8)) : make_uint4(0u, 0u, 0u, 0u);
         };
-        if constexpr (!SRC) {
+        if constexpr (!SRC && GATE == 0) {
 #pragma unroll
           for (int q = 0; q < 8; ++q) bv[q] = bias8(q);
         }
@@ -466,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
 #pragma unroll
               for (int q = 0; q < 4; ++q) add8(v + 8 * q, bias8(4 * hh + q));
             }
-          } else {
+          } else if constexpr (GATE == 0) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) add8(v + 8 * q, bv[4 * hh + q]);
           }
@@ -523,8 +597,28 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const int row = row0 + 4 * k + (lane >> 3);
-          if (row < M && ccol < N)
-            *reinterpret_cast<uint4*>(d + (long long)row * ldd + ccol) = *reinterpret_cast<const uint4*>((k & 1 ? coal1 : coal0) + 4 * k * kPitch);
+          if (row < M && ccol < N) {
+            const uint4 v = *reinterpret_cast<const uint4*>((k & 1 ? coal1 : coal0) + 4 * k * kPitch);
+            if constexpr (GATE == 2) {
+              const uint32_t a[4] = {gv[k].x, gv[k].y, gv[k].z, gv[k].w}, b[4] = {uv[k].x, uv[k].y, uv[k].z, uv[k].w}, e[4] = {v.x, v.y, v.z, v.w};
+              uint32_t og[4], ou[4], oh[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float g0, u0, g1, u1;
+                swiglu_grad(bf16_lo(a[i]), bf16_lo(b[i]), bf16_lo(e[i]), g0, u0);
+                swiglu_grad(bf16_hi(a[i]), bf16_hi(b[i]), bf16_hi(e[i]), g1, u1);
+                og[i] = pack_bf16(g0, g1);
+                ou[i] = pack_bf16(u0, u1);
+                oh[i] = pack_bf16(swiglu(bf16_lo(a[i]), bf16_lo(b[i])), swiglu(bf16_hi(a[i]), bf16_hi(b[i])));
+              }
+              __nv_bfloat16* to = P.dgu + (long long)row * P.lddgu + ccol;
+              *reinterpret_cast<uint4*>(to) = make_uint4(og[0], og[1], og[2], og[3]);
+              *reinterpret_cast<uint4*>(to + P.gate_cols) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+              if (d) *reinterpret_cast<uint4*>(d + (long long)row * ldd + ccol) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
+            } else {
+              *reinterpret_cast<uint4*>(d + (long long)row * ldd + ccol) = v;
+            }
+          }
         }
         __syncwarp();
       }
@@ -700,9 +794,9 @@ long long makespan(const Item* it, int n, const TileShape* const* sh, int units,
   return best + epi;
 }
 
-template <bool PAIR, int MAXJ, bool SRC, bool FUN, bool FILL = false>
+template <bool PAIR, int MAXJ, bool SRC, bool FUN, bool FILL = false, int GATE = 0>
 int launch_local(const Params<MAXJ>& P, cudaStream_t stream) {
-  if (ensure_smem<local_gemm_kernel<PAIR, MAXJ, SRC, FUN, FILL>>(kSmem) != cudaSuccess) return lfail("cudaFuncSetAttribute failed");
+  if (ensure_smem<local_gemm_kernel<PAIR, MAXJ, SRC, FUN, FILL, GATE>>(kSmem) != cudaSuccess) return lfail("cudaFuncSetAttribute failed");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(PAIR ? 2 * P.units : P.units);
   cfg.blockDim = dim3(kThreads);
@@ -722,7 +816,7 @@ int launch_local(const Params<MAXJ>& P, cudaStream_t stream) {
   }
   cfg.attrs = at;
   cfg.numAttrs = nat;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, local_gemm_kernel<PAIR, MAXJ, SRC, FUN, FILL>, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, local_gemm_kernel<PAIR, MAXJ, SRC, FUN, FILL, GATE>, P);
   return e == cudaSuccess ? 0 : lfail(std::string("launch local_gemm_kernel: ") + cudaGetErrorString(e));
 }
 
@@ -734,6 +828,8 @@ long long choose(const Item* it, int n, int pair_policy, int n_sm, const TileSha
   long long best = -1;
   for (int s = 0; s < 4; s += 2) {
     const TileShape *wide = &kShapes[s], *narrow = &kShapes[s + 1];
+    // gate and up need 64 columns of a tile each at least: two of the epilogue's warps share its rows, 32 columns a piece
+    if (n == 1 && it[0].g->gate == 1 && narrow->bn < 128) narrow = wide;
     const int units = wide->pair ? n_sm / 2 : n_sm;
     if (!units || pair_policy == (wide->pair ? 0 : 1)) continue;
     auto consider = [&] {
@@ -801,9 +897,14 @@ int run(const Item* it, int n, int pair_policy, unsigned long long* status, unsi
     J.bn = best_sh[best_ord[q]]->bn;
     const int rows_b = pair ? J.bn / 2 : J.bn;
     widest = std::max(widest, rows_b);
-    if (operand_map(&J.mb, &J.b3, x.b, x.N, x.K, x.ldb, x.b_mn, rows_b)) return -1;
+    if (operand_map(&J.mb, &J.b3, x.b, x.N, x.K, x.ldb, x.b_mn, x.gate == 1 ? J.bn / 2 : rows_b)) return -1;
     J.b_mn = (unsigned char)x.b_mn;
     J.N = x.N; J.tiles_n = (x.N + J.bn - 1) / J.bn;
+    if (x.gate) {
+      P.gate_cols = x.gate == 1 ? x.N / 2 : x.N;
+      P.gu = reinterpret_cast<__nv_bfloat16*>(x.gu); P.ldgu = x.ldgu;
+      P.dgu = reinterpret_cast<__nv_bfloat16*>(x.dgu); P.lddgu = x.lddgu;
+    }
     // Every group reads all of B again, so a wide output takes 16 rows a group while their part of A still stays in L2 beside
     // it: forward 4096 x 2048 -> 50304 563 -> 546 us, 8192 rows 1147 -> 1103.  Not for a tall one (weight gradient of 50304 x
     // 2048 over 4096 1238 -> 1298 us) nor a long contraction (8192^3 724 -> 740).
@@ -833,6 +934,10 @@ int run(const Item* it, int n, int pair_policy, unsigned long long* status, unsi
   if (fill) {
     if (src || fun) return lfail("local_gemm: rows in use go with plain jobs only");
     return pair ? launch_local<true, MAXJ, false, false, true>(P, stream) : launch_local<false, MAXJ, false, false, true>(P, stream);
+  }
+  if constexpr (MAXJ == 3) {
+    if (it[0].g->gate == 1) return pair ? launch_local<true, MAXJ, false, false, false, 1>(P, stream) : launch_local<false, MAXJ, false, false, false, 1>(P, stream);
+    if (it[0].g->gate == 2) return pair ? launch_local<true, MAXJ, false, false, false, 2>(P, stream) : launch_local<false, MAXJ, false, false, false, 2>(P, stream);
   }
 #define RTP_LOCAL(SRC, FUN) (pair ? launch_local<true, MAXJ, SRC, FUN>(P, stream) : launch_local<false, MAXJ, SRC, FUN>(P, stream))
   return src ? (fun ? RTP_LOCAL(true, true) : RTP_LOCAL(true, false)) : (fun ? RTP_LOCAL(false, true) : RTP_LOCAL(false, false));
@@ -873,6 +978,11 @@ bool local_gemm_ok(const LocalGemm& g) {
   if (g.part < 0 || (g.part && ((g.K + 63) / 64 + g.part - 1) / g.part * (g.part - 1) >= (g.K + 63) / 64)) return false;
   if (g.part && (g.c || g.bias || g.act || g.mask || g.drop_p > 0.f || g.bsum_add)) return false;
   if ((g.m_fill || g.k_fill) && (g.c || g.act || g.mask || g.drop_p > 0.f || g.bsum_add || g.part)) return false;
+  if (g.gate) {
+    if (g.c || g.bias || g.act || g.mask || g.drop_p > 0.f || g.bsum || g.part || g.m_fill || g.k_fill) return false;
+    if (!al16(g.gu) || !al16(g.dgu) || g.ldgu % 8 || g.lddgu % 8) return false;
+    if (g.gate == 1 ? (g.b_mn || g.N % 16 || !g.d) : (!g.gu || !g.dgu)) return false;
+  }
   return !g.bsum || g.a_mn;
 }
 
@@ -880,7 +990,7 @@ int local_gemm(const LocalGemm* jobs, int n, int pair_policy, unsigned long long
                cudaStream_t stream) {
   if (n < 1 || n > kLocalMaxJobs) return lfail("local_gemm: number of jobs out of range");
   for (int i = 0; i < n; ++i)
-    if (!local_gemm_ok(jobs[i])) return lfail("local_gemm: operand not aligned to 16 bytes, or N not a multiple of 8");
+    if (!local_gemm_ok(jobs[i]) || (jobs[i].gate && n > 1)) return lfail("local_gemm: operand not aligned to 16 bytes, or N not a multiple of 8");
   Item it[kMaxItems];
   const int m = items_of(jobs, n, it);
   if (m < 0) return lfail("local_gemm: too many column sums");

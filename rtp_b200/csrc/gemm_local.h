@@ -34,6 +34,15 @@ struct LocalGemm {
   // multiple of 64 are finite.  A launch with one of them has no c, mask, activation or dropout.
   const int* m_fill;
   const int* k_fill;
+  // A gated feed-forward block's own epilogues; such a job is alone in its launch and has no c, bias, act, mask, dropout, bsum, part or
+  // fill.  F = columns of d.
+  // 1: B is [2 F, K] (K-major), the gate's rows before the up projection's, N = 2 F.  d = silu(A gate^T) * (A up^T); gu (may be null)
+  //    receives the two projections [M, 2 F].
+  // 2: N = F, the product is the gradient of d: gu [M, 2 F] is read, dgu [M, 2 F] receives the gradients of the two projections and d
+  //    (may be null) silu(gate) * up once more.
+  int gate;
+  void* gu; long long ldgu;
+  void* dgu; long long lddgu;
 };
 
 // Whether the local kernels take this job (16-byte aligned rows, N a multiple of 8).

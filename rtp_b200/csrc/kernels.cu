@@ -1364,7 +1364,7 @@ __global__ void swiglu_fwd_kernel(const __nv_bfloat16* g, const __nv_bfloat16* u
   unpack8(*reinterpret_cast<const uint4*>(g + r * ld + c), a);
   unpack8(*reinterpret_cast<const uint4*>(u + r * ld + c), b);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) a[k] = a[k] / (1.f + __expf(-a[k])) * b[k];
+  for (int k = 0; k < 8; ++k) a[k] = rtp::swiglu(a[k], b[k]);
   *reinterpret_cast<uint4*>(y + r * cols + c) = pack8(a);
 }
 __global__ void swiglu_bwd_kernel(const __nv_bfloat16* g, const __nv_bfloat16* u, long long ld, const __nv_bfloat16* dy,
@@ -1379,12 +1379,7 @@ __global__ void swiglu_bwd_kernel(const __nv_bfloat16* g, const __nv_bfloat16* u
   unpack8(*reinterpret_cast<const uint4*>(u + r * ld + c), b);
   unpack8(*reinterpret_cast<const uint4*>(dy + r * cols + c), d);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float sg = 1.f / (1.f + __expf(-a[k]));
-    const float silu = a[k] * sg;
-    ou[k] = d[k] * silu;
-    og[k] = d[k] * b[k] * (sg + silu * (1.f - sg));
-  }
+  for (int k = 0; k < 8; ++k) rtp::swiglu_grad(a[k], b[k], d[k], og[k], ou[k]);
   *reinterpret_cast<uint4*>(dg + r * ldo + c) = pack8(og);
   *reinterpret_cast<uint4*>(du + r * ldo + c) = pack8(ou);
 }

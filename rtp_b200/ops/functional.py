@@ -284,6 +284,21 @@ def swiglu_packed(y, nshard=1):
     return swiglu(*_split_packed(y, 2, nshard))
 
 
+def gated_mlp(x, w_gate_up, w_down):
+    """Gated feed-forward block ``(silu(x Wg^T) * (x Wu^T)) Wd^T``: ``x`` [..., D], ``w_gate_up`` [2 * F, D] (the rows of ``Wg`` before those
+    of ``Wu``), ``w_down`` [O, F] -> [..., O].
+
+    bf16 CUDA tensors whose sizes are multiples of 8 run on the tcgen05 GEMM kernel with the activation and the product in its epilogue
+    (``ops/mlp.py``): sums in fp32; gate, up, their product and their gradients are rounded to bf16, as the operands of the
+    products behind them."""
+    from . import mlp
+    if get_backend() != "functional" and x.dim() and w_gate_up.dim() == 2 and w_down.dim() == 2 and mlp.kernel_takes(x, w_gate_up, w_down):
+        return mlp.gated_mlp(x, w_gate_up, w_down)
+    mlp.check_args(x, w_gate_up, w_down)
+    g, u = F.linear(x, w_gate_up).chunk(2, dim=-1)
+    return F.linear(F.silu(g) * u, w_down)
+
+
 class _RopeAttnPackedFn(torch.autograd.Function):
     """Causal self-attention of a packed projection [B * S, 3 * D] with rotary embedding of q and k.  Forward makes one rotated
     copy of the projection, which the flash kernels read in place; backward turns the q and k gradients back inside the
