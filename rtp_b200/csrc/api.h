@@ -39,10 +39,11 @@ typedef struct {
   void* gu;                                   // the two projections, for the backward (null: not kept)
   void* h;                                    // workspace
   void* y;
+  int whole;                                  // 1: sums in the order of separate layers (products of few rows are not cut into slices)
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;   // rtp_gated_fwd_scratch() bytes, 16-byte aligned (none: null)
 } RtpGatedFwd;
-int rtp_gated_fwd(const RtpGatedFwd* args, void* stream);                 // two launches, three with scratch
+int rtp_gated_fwd(const RtpGatedFwd* args, void* stream);                 // two launches, and one for each product in slices
 unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* args);
 typedef struct {
   int T, D, F, O;
@@ -54,6 +55,7 @@ typedef struct {
   void* dgu;                                  // workspace
   void* h;                                    // workspace, needed for dw_d
   void *dx, *dw_gu, *dw_d;                    // each may be null
+  int whole;
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;
 } RtpGatedBwd;

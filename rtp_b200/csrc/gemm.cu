@@ -1159,20 +1159,6 @@ int gated_sizes(int T, int D, int F, int O) {
   if (F > (1 << 29)) return fail("gated feed-forward: too many columns");
   return 0;
 }
-rtp::LocalGemm gated_down(const RtpGatedFwd& a) {
-  rtp::LocalGemm j = {};
-  j.a = a.h; j.lda = a.F; j.b = a.w_d; j.ldb = a.ld_d;
-  j.M = a.T; j.N = a.O; j.K = a.F;
-  j.d = a.y; j.ldd = a.O;
-  return j;
-}
-rtp::LocalGemm gated_dx(const RtpGatedBwd& a) {
-  rtp::LocalGemm j = {};
-  j.a = a.dgu; j.lda = 2ll * a.F; j.b = a.w_gu; j.ldb = a.ld_gu; j.b_mn = 1;
-  j.M = a.T; j.N = a.D; j.K = 2 * a.F;
-  j.d = a.dx; j.ldd = a.D;
-  return j;
-}
 // Slices of the contraction of a product with few rows: its few tiles would read the weights with a few SMs (8 x 8192 -> 2048: 16 tiles
 // of 128 k-blocks).  As many as fill the SMs, of six k-blocks or more; none (0) where the tiles fill half of the SMs or the launch
 // that adds the slices up would take longer than they save.
@@ -1182,22 +1168,76 @@ int few_row_slices(const rtp::LocalGemm& w) {
   const int want = (int)std::min<long long>(sm_count() / tiles, kb / 6), per = (int)((kb + want - 1) / want);
   return (int)((kb + per - 1) / per);
 }
-unsigned long long split_bytes(const rtp::LocalGemm& w) { return (unsigned long long)few_row_slices(w) * part_stride(w) * 4; }
-// Runs the jobs, of which `w` (may be null) is split if it is one to be split.
-int run_split(rtp::LocalGemm* jobs, int n, rtp::LocalGemm* w, void* scratch, unsigned long long bytes, unsigned long long* status, void* stream) {
-  const int slices = w ? few_row_slices(*w) : 0;
-  if (!slices) return run_local(jobs, n, status, 0, stream);
-  if (!scratch || bytes < split_bytes(*w) || (reinterpret_cast<uintptr_t>(scratch) & 15))
+// The products of a launch (three at most), some of them in slices of their contraction (0: none).
+struct SplitJobs {
+  rtp::LocalGemm job[3];
+  int slices[3], n;
+  void add(const rtp::LocalGemm& w, int k) { job[n] = w; slices[n++] = k; }
+  unsigned long long bytes() const {
+    unsigned long long b = 0;
+    for (int i = 0; i < n; ++i) b += (unsigned long long)slices[i] * part_stride(job[i]) * 4;
+    return b;
+  }
+};
+int run_split(SplitJobs& s, void* scratch, unsigned long long bytes, unsigned long long* status, void* stream) {
+  if (!s.n) return 0;
+  const unsigned long long need = s.bytes();
+  if (need && (!scratch || bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15)))
     return fail("gated feed-forward: workspace missing, too small or not aligned to 16 bytes");
-  void* d = w->d;
-  const long long len = (long long)w->M * w->N, stride = part_stride(*w);
-  w->part = slices;
-  w->part_stride = stride;
-  w->d = scratch; w->ldd = w->N;
-  if (run_local(jobs, n, status, 0, stream)) return -1;
-  if (rtp::local_reduce(reinterpret_cast<const float*>(scratch), slices, stride, d, len, 0, nullptr, 0, (cudaStream_t)stream))
-    return fail(rtp::local_gemm_error());
+  float* part = reinterpret_cast<float*>(scratch);
+  void* d[3];
+  for (int i = 0; i < s.n; ++i) {
+    if (!s.slices[i]) continue;
+    rtp::LocalGemm& w = s.job[i];
+    d[i] = w.d;
+    w.part = s.slices[i];
+    w.part_stride = part_stride(w);
+    w.d = part; w.ldd = w.N;
+    part += w.part * w.part_stride;
+  }
+  if (run_local(s.job, s.n, status, 0, stream)) return -1;
+  for (int i = 0; i < s.n; ++i) {
+    const rtp::LocalGemm& w = s.job[i];
+    if (s.slices[i] && rtp::local_reduce(reinterpret_cast<const float*>(w.d), w.part, w.part_stride, d[i], (long long)w.M * w.N, 0, nullptr,
+                                         0, (cudaStream_t)stream))
+      return fail(rtp::local_gemm_error());
+  }
   return 0;
+}
+SplitJobs gated_down(const RtpGatedFwd& a) {
+  SplitJobs s = {};
+  rtp::LocalGemm j = {};
+  j.a = a.h; j.lda = a.F; j.b = a.w_d; j.ldb = a.ld_d;
+  j.M = a.T; j.N = a.O; j.K = a.F;
+  j.d = a.y; j.ldd = a.O;
+  s.add(j, a.whole ? 0 : few_row_slices(j));
+  return s;
+}
+// Both weight gradients, in slices by the rule of a rotated layer's, and the input gradient.
+SplitJobs gated_grads(const RtpGatedBwd& a) {
+  SplitJobs s = {};
+  if (a.dw_gu) {
+    rtp::LocalGemm w = {};
+    w.a = a.dgu; w.lda = 2ll * a.F; w.a_mn = 1; w.b = a.x; w.ldb = a.ldx; w.b_mn = 1;
+    w.M = 2 * a.F; w.N = a.D; w.K = a.T;
+    w.d = a.dw_gu; w.ldd = a.D;
+    s.add(w, splits_wgrad(w) ? wgrad_slices(w) : 0);
+  }
+  if (a.dw_d) {
+    rtp::LocalGemm w = {};
+    w.a = a.dy; w.lda = a.ldy; w.a_mn = 1; w.b = a.h; w.ldb = a.F; w.b_mn = 1;
+    w.M = a.O; w.N = a.F; w.K = a.T;
+    w.d = a.dw_d; w.ldd = a.F;
+    s.add(w, splits_wgrad(w) ? wgrad_slices(w) : 0);
+  }
+  if (a.dx) {
+    rtp::LocalGemm j = {};
+    j.a = a.dgu; j.lda = 2ll * a.F; j.b = a.w_gu; j.ldb = a.ld_gu; j.b_mn = 1;
+    j.M = a.T; j.N = a.D; j.K = 2 * a.F;
+    j.d = a.dx; j.ldd = a.D;
+    s.add(j, a.whole ? 0 : few_row_slices(j));
+  }
+  return s;
 }
 int local_expert_fwd(const RtpRing& R, const RtpExpertFwd& op, rtp::LocalGemm* j) {
   if (R.world != 1 || g_trace || op.n_local < 1 || op.n_local > rtp::kLocalMaxJobs) return 0;
@@ -1600,42 +1640,30 @@ int rtp_gemm(const RtpGemmArgs* a, void* stream) {
 int rtp_gated_fwd(const RtpGatedFwd* a, void* stream) {
   if (gated_sizes(a->T, a->D, a->F, a->O)) return -1;
   if (!a->h || !a->y) return fail("gated feed-forward: outputs missing");
-  rtp::LocalGemm up = {}, down = gated_down(*a);
+  rtp::LocalGemm up = {};
   up.a = a->x; up.lda = a->ldx; up.b = a->w_gu; up.ldb = a->ld_gu;
   up.M = a->T; up.N = 2 * a->F; up.K = a->D;
   up.d = a->h; up.ldd = a->F;
   up.gate = 1; up.gu = a->gu; up.ldgu = 2ll * a->F;
-  return run_local(&up, 1, a->status, 0, stream) || run_split(&down, 1, &down, a->scratch, a->scratch_bytes, a->status, stream) ? -1 : 0;
+  SplitJobs down = gated_down(*a);
+  return run_local(&up, 1, a->status, 0, stream) || run_split(down, a->scratch, a->scratch_bytes, a->status, stream) ? -1 : 0;
 }
-unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* a) { return a->T > 0 && a->F > 0 && a->O > 0 ? split_bytes(gated_down(*a)) : 0; }
+unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* a) { return a->T > 0 && a->F > 0 && a->O > 0 ? gated_down(*a).bytes() : 0; }
 
 int rtp_gated_bwd(const RtpGatedBwd* a, void* stream) {
   if (gated_sizes(a->T, a->D, a->F, a->O)) return -1;
   if (!a->gu || !a->dgu || (a->dw_d && !a->h)) return fail("gated feed-forward: workspace missing");
-  rtp::LocalGemm h = {}, j[3] = {}, *dx = nullptr;
+  rtp::LocalGemm h = {};
   h.a = a->dy; h.lda = a->ldy; h.b = a->w_d; h.ldb = a->ld_d; h.b_mn = 1;
   h.M = a->T; h.N = a->F; h.K = a->O;
   h.d = a->dw_d ? a->h : nullptr; h.ldd = a->F;
   h.gate = 2; h.gu = const_cast<void*>(a->gu); h.ldgu = 2ll * a->F; h.dgu = a->dgu; h.lddgu = 2ll * a->F;
   if (run_local(&h, 1, a->status, 0, stream)) return -1;
-  int n = 0;
-  if (a->dw_gu) {
-    rtp::LocalGemm& w = j[n++];
-    w.a = a->dgu; w.lda = 2ll * a->F; w.a_mn = 1; w.b = a->x; w.ldb = a->ldx; w.b_mn = 1;
-    w.M = 2 * a->F; w.N = a->D; w.K = a->T;
-    w.d = a->dw_gu; w.ldd = a->D;
-  }
-  if (a->dw_d) {
-    rtp::LocalGemm& w = j[n++];
-    w.a = a->dy; w.lda = a->ldy; w.a_mn = 1; w.b = a->h; w.ldb = a->F; w.b_mn = 1;
-    w.M = a->O; w.N = a->F; w.K = a->T;
-    w.d = a->dw_d; w.ldd = a->F;
-  }
-  if (a->dx) *(dx = &j[n++]) = gated_dx(*a);
-  return n ? run_split(j, n, dx, a->scratch, a->scratch_bytes, a->status, stream) : 0;
+  SplitJobs grads = gated_grads(*a);
+  return run_split(grads, a->scratch, a->scratch_bytes, a->status, stream);
 }
 unsigned long long rtp_gated_bwd_scratch(const RtpGatedBwd* a) {
-  return a->dx && a->T > 0 && a->F > 0 && a->D > 0 ? split_bytes(gated_dx(*a)) : 0;
+  return a->T > 0 && a->D > 0 && a->F > 0 && a->O > 0 ? gated_grads(*a).bytes() : 0;
 }
 
 int rtp_gemm_batched(const RtpGemmBatched* a, void* stream) {

@@ -31,10 +31,10 @@ constexpr int kThreads = 256;
 constexpr int kMaxTile = 64;              // tokens of a block
 constexpr int kMaxTrig = 2048;            // their (cosine, sine) pairs: 16 KB
 
-struct Side {                             // q or k: [B, S, heads, hd] views in, contiguous out
+struct Side {                             // q or k: [B, S, heads, hd] views in and out (out may be in)
   const void* in;
   void* out;
-  long long sb, ss, sh;
+  long long sb, ss, sh, osb, oss, osh;
   int heads;
 };
 struct Params {
@@ -63,7 +63,7 @@ struct alignas(sizeof(T) * V) Vec { T e[V]; };
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Params p) {
   __shared__ __align__(16) float s_cos[kMaxTrig], s_sin[kMaxTrig];
-  __shared__ long long s_q[kMaxTile], s_k[kMaxTile];
+  __shared__ long long s_at[2][2][kMaxTile];                // [q, k][in, out]: where a token begins
   pdl_prologue();
   const long long t0 = blockIdx.x * (long long)p.tile;
   const int n = (int)min((long long)p.tile, p.tokens - t0), half = p.rot >> 1, tid = threadIdx.x;
@@ -80,8 +80,10 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
   for (int t = tid; t < n; t += kThreads) {
     const long long b = (t0 + t) / p.S, s = t0 + t - b * p.S;
-    s_q[t] = b * p.q.sb + s * p.q.ss;
-    s_k[t] = b * p.k.sb + s * p.k.ss;
+    s_at[0][0][t] = b * p.q.sb + s * p.q.ss;
+    s_at[0][1][t] = b * p.q.osb + s * p.q.oss;
+    s_at[1][0][t] = b * p.k.sb + s * p.k.ss;
+    s_at[1][1][t] = b * p.k.osb + s * p.k.oss;
   }
   __syncthreads();
   const int row0 = tid / p.per_head, j = tid - row0 * p.per_head;
@@ -93,8 +95,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const bool is_q = h < p.q.heads;
     const Side& sd = is_q ? p.q : p.k;
     const int hh = is_q ? h : h - p.q.heads;
-    const T* in = reinterpret_cast<const T*>(sd.in) + (is_q ? s_q[t] : s_k[t]) + hh * sd.sh;
-    T* out = reinterpret_cast<T*>(sd.out) + ((t0 + t) * sd.heads + hh) * p.hd;
+    const T* in = reinterpret_cast<const T*>(sd.in) + s_at[!is_q][0][t] + hh * sd.sh;
+    T* out = reinterpret_cast<T*>(sd.out) + s_at[!is_q][1][t] + hh * sd.osh;
     const float *cs = s_cos + t * half, *sn = s_sin + t * half;
     if constexpr (HALF) {
       const int c = j * V;
@@ -143,12 +145,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 int access_bytes(const RtpRotary& a, int size) {
   for (int bytes = 16; bytes > size; bytes >>= 1) {
     const int v = bytes / size;
-    auto fits = [&](const void* in, const void* out, long long sb, long long ss, long long sh) {
-      return ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & (uintptr_t)(bytes - 1)) == 0 && sb % v == 0 &&
-             ss % v == 0 && sh % v == 0;
+    auto fits = [&](const void* x, long long sb, long long ss, long long sh) {
+      return (reinterpret_cast<uintptr_t>(x) & (uintptr_t)(bytes - 1)) == 0 && sb % v == 0 && ss % v == 0 && sh % v == 0;
     };
     if (a.hd % v || (a.half_layout ? a.rot / 2 : a.rot) % v) continue;
-    if (!fits(a.q, a.qo, a.q_sb, a.q_ss, a.q_sh) || (a.k_heads && !fits(a.k, a.ko, a.k_sb, a.k_ss, a.k_sh))) continue;
+    if (a.q_heads && (!fits(a.q, a.q_sb, a.q_ss, a.q_sh) || !fits(a.qo, a.qo_sb, a.qo_ss, a.qo_sh))) continue;
+    if (a.k_heads && (!fits(a.k, a.k_sb, a.k_ss, a.k_sh) || !fits(a.ko, a.ko_sb, a.ko_ss, a.ko_sh))) continue;
     return bytes;
   }
   return size;
@@ -175,8 +177,8 @@ int rtp_rotary(const RtpRotary* a, void* stream) {
   if (!tokens || !heads) return 0;
   const int size = a->dtype == 2 ? 4 : 2, bytes = access_bytes(*a, size), v = bytes / size;
   Params P = {};
-  P.q = Side{a->q, a->qo, a->q_sb, a->q_ss, a->q_sh, a->q_heads};
-  P.k = Side{a->k, a->ko, a->k_sb, a->k_ss, a->k_sh, a->k_heads};
+  P.q = Side{a->q, a->qo, a->q_sb, a->q_ss, a->q_sh, a->qo_sb, a->qo_ss, a->qo_sh, a->q_heads};
+  P.k = Side{a->k, a->ko, a->k_sb, a->k_ss, a->k_sh, a->ko_sb, a->ko_ss, a->ko_sh, a->k_heads};
   P.positions = a->positions; P.pb = a->pos_sb; P.ps = a->pos_ss; P.pos64 = a->pos64;
   P.freqs = a->freqs; P.magnitude = a->magnitude; P.sign = a->backward ? -1.f : 1.f;
   P.tokens = tokens; P.S = a->S; P.hd = a->hd; P.rot = a->rot;

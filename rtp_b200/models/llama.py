@@ -2,7 +2,8 @@
 
 Rotation plan per block: packed QKV projection = column-rotated ``D -> 3D`` whose shard rows are
 ``[q_r; k_r; v_r]`` (heads/N heads per shard), attention over all heads locally (each rank holds the full
-projection of its own batch once the N column blocks are assembled), output projection = row-rotated ``D -> D``;
+projection of its own batch once the N column blocks are assembled), optionally over a window of recent tokens and the
+first few, output projection = row-rotated ``D -> D``;
 SwiGLU = column-rotated packed gate/up ``D -> 2F`` (shard rows ``[gate_r; up_r]``) and row-rotated ``F -> D``.
 Embedding ``[V, D/N]`` and LM head ``[V/N, D]`` rotate as well.  Activations are ``[batch, seq, dim]``."""
 from dataclasses import dataclass
@@ -13,7 +14,9 @@ import torch.nn as nn
 from ..module.embedding import ParallelEmbedding
 from ..module.linear import ColumnParallelLinear, RowParallelLinear
 from ..parallel.context import get_context
+from ..parallel import fused
 from ..ops import functional as FO
+from ..ops.rotary import LAYOUTS, SCALINGS, rotary_frequencies, rotary_magnitude
 
 
 @dataclass
@@ -28,6 +31,29 @@ class LlamaConfig:
     norm_eps: float = 1e-5
     init_std: float = 0.02
     loss_chunk_rows: int = 0     # > 0: LM head + cross-entropy this many tokens at a time (no full logits)
+    # attention over the last `window` tokens and the first `sinks` (0: over all earlier ones)
+    window: int = 0
+    sinks: int = 0
+    # rotary positions: layout of the pairs, rotated part of a head (0: all of it), stretched frequencies (ops.rotary.rotary_frequencies)
+    rope_layout: str = "interleaved"
+    rotary_dim: int = 0
+    rope_scaling: str = "none"
+    rope_factor: float = 1.0
+    rope_original_length: int = 4096
+
+    def __post_init__(self):
+        if self.window < 0 or self.sinks < 0 or (self.sinks and not self.window):
+            raise ValueError(f"window and sinks must not be negative, and sinks go with a window: got {self.window} and {self.sinks}")
+        if self.rope_layout not in LAYOUTS or self.rope_scaling not in SCALINGS:
+            raise ValueError(f"rope_layout must be one of {LAYOUTS} and rope_scaling one of {SCALINGS}, got {self.rope_layout!r} and {self.rope_scaling!r}")
+        if self.rotary_dim < 0 or self.rotary_dim % 2 or self.rotary_dim > self.d_model // self.n_heads:
+            raise ValueError(f"rotary_dim must be even and lie inside the head, got {self.rotary_dim}")
+
+    @property
+    def table_rope(self):
+        """Whole heads in the interleaved layout with plain frequencies under full causal attention: the packed kernels' case."""
+        return not self.window and self.rope_layout == "interleaved" and self.rotary_dim in (0, self.d_model // self.n_heads) and \
+            self.rope_scaling == "none"
 
     @staticmethod
     def llama_13b():
@@ -78,21 +104,33 @@ class LlamaBlock(nn.Module):
         self.gate_up = ColumnParallelLinear(cfg.d_model, 2 * cfg.d_ff, packed_parts=2, **kw)
         self.down = RowParallelLinear(cfg.d_ff, cfg.d_model, **kw)
 
-    def forward(self, x, cos, sin):
+    def _table_attention(self, qkv, cos, sin):
         cfg = self.cfg
-        B, S, D = x.shape
-        hd = D // cfg.n_heads
-        qkv = self.qkv(self.norm1(x))
+        B, S, W = qkv.shape
         a = FO.rope_attention_packed(qkv, cos, sin, cfg.n_heads, self.N)
         if a is None:
+            heads = (B, S, cfg.n_heads, W // (3 * cfg.n_heads))
             q, k, v = FO._split_packed(qkv, 3, self.N)
-            q = apply_rope(q.view(B, S, cfg.n_heads, hd), cos, sin)
-            k = apply_rope(k.view(B, S, cfg.n_heads, hd), cos, sin)
-            v = v.view(B, S, cfg.n_heads, hd)
-            a = FO.causal_attention(q, k, v).reshape(B, S, D)      # [B, S, H, hd]
-        x = x + self.proj(a)
-        x = x + self.down(FO.swiglu_packed(self.gate_up(self.norm2(x)), self.N))
-        return x
+            q = apply_rope(q.view(heads), cos, sin)
+            k = apply_rope(k.view(heads), cos, sin)
+            a = FO.causal_attention(q, k, v.view(heads)).reshape(B, S, W // 3)      # [B, S, H, hd]
+        return a
+
+    def _window_attention(self, qkv, positions, freqs):
+        cfg = self.cfg
+        if self.N > 1:                                             # the shards' column groups side by side -> q | k | v
+            qkv = torch.cat(FO._split_packed(qkv, 3, self.N), dim=-1)
+        return FO.rotary_window_attention(qkv, positions, freqs, cfg.n_heads, layout=cfg.rope_layout,
+                                          magnitude=rotary_magnitude(cfg.rope_scaling, cfg.rope_factor),
+                                          window=cfg.window or None, sinks=cfg.sinks)
+
+    def forward(self, x, *rope):
+        """``rope``: the cosine and sine tables, or positions and frequencies (see ``LlamaConfig.table_rope``)."""
+        qkv = self.qkv(self.norm1(x))
+        x = x + self.proj((self._table_attention if self.cfg.table_rope else self._window_attention)(qkv, *rope))
+        h = self.norm2(x)
+        y = fused.gated_mlp(self.gate_up, self.down, h)
+        return x + (self.down(FO.swiglu_packed(self.gate_up(h), self.N)) if y is None else y)
 
 
 class Llama(nn.Module):
@@ -110,10 +148,17 @@ class Llama(nn.Module):
 
     def forward(self, ids, targets=None):
         B, S = ids.shape
-        cos, sin = rope_tables(S, self.cfg.d_model // self.cfg.n_heads, self.cfg.rope_theta, ids.device)
+        cfg = self.cfg
+        hd = cfg.d_model // cfg.n_heads
+        if cfg.table_rope:
+            rope = rope_tables(S, hd, cfg.rope_theta, ids.device)
+        else:
+            rope = (torch.arange(S, device=ids.device),
+                    rotary_frequencies(cfg.rotary_dim or hd, cfg.rope_theta, cfg.rope_scaling, cfg.rope_factor, cfg.rope_original_length,
+                                       device=ids.device))
         x = self.tok(ids)
         for blk in self.blocks:
-            x = blk(x, cos, sin)
+            x = blk(x, *rope)
         if targets is not None and self.cfg.loss_chunk_rows > 0:
             # head and loss chunk by chunk: the [tokens, vocab] logits never exist as a whole
             return FO.chunked_head_loss(self.norm(x), targets, self.head, self.cfg.loss_chunk_rows)

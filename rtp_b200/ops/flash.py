@@ -297,16 +297,20 @@ def _window_fwd(q, k, v, window, sinks, sm_scale, want_lse):
     return q, k, v, o, lse
 
 
-def _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale):
+def _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale, out=None):
+    """``out``: (dq, dk, dv) views to write to, as long as there are as many queries as keys."""
     if q.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(q.device):
-            return _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale)
+            return _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale, out)
     do = _addressable(do)
-    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    # blocks of keys that come before every window and hold no sink are not written
-    unseen = max(0, k.shape[1] - q.shape[1] - window + 1) // 128 > -(-min(sinks, k.shape[1]) // 128)
-    new = torch.zeros_like if unseen else torch.empty_like
-    dk, dv = (new(t, memory_format=torch.contiguous_format) for t in (k, v))
+    if out is None:
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        # blocks of keys that come before every window and hold no sink are not written
+        unseen = max(0, k.shape[1] - q.shape[1] - window + 1) // 128 > -(-min(sinks, k.shape[1]) // 128)
+        new = torch.zeros_like if unseen else torch.empty_like
+        dk, dv = (new(t, memory_format=torch.contiguous_format) for t in (k, v))
+    else:
+        dq, dk, dv = out
     delta = torch.empty_like(lse)
     a = _window_args(q, k, v, o, lse, window, sinks, sm_scale)
     f = a.f
@@ -345,3 +349,40 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _WindowFn.apply(q, k, v, window, sinks, sm_scale)
     return _window_fwd(q, k, v, window, sinks, sm_scale, False)[3]
+
+
+class _RotaryWindowPackedFn(torch.autograd.Function):
+    """Windowed self-attention of a packed projection [B, S, (H + 2 Hk) * hd] with rotary positions.  q and k are turned into tensors of
+    their own, v is read where it lies; backward writes all three gradients into one packed tensor and turns those of q and k back
+    inside it, without a zero-filled gradient for each slice."""
+
+    @staticmethod
+    def forward(ctx, qkv, positions, freqs, half, magnitude, H, Hk, hd, window, sinks):
+        from .rotary import _rotate
+        q, k, v = qkv.view(*qkv.shape[:2], H + 2 * Hk, hd).split((H, Hk, Hk), dim=2)
+        q, k = _rotate(q, k, positions, freqs, half, magnitude, False)
+        q, k, v, o, lse = _window_fwd(q, k, v, window, sinks, hd ** -0.5, True)
+        ctx.save_for_backward(q, k, v, o, lse, positions, freqs)
+        ctx.cfg = (half, magnitude, window, sinks)
+        return o.view(*qkv.shape[:2], H * hd)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        from .rotary import _rotate
+        q, k, v, o, lse, positions, freqs = ctx.saved_tensors
+        half, magnitude, window, sinks = ctx.cfg
+        B, S, H, hd = q.shape
+        Hk = k.shape[2]
+        dqkv = q.new_empty(B, S, (H + 2 * Hk) * hd)
+        dq, dk, dv = dqkv.view(B, S, H + 2 * Hk, hd).split((H, Hk, Hk), dim=2)
+        _window_bwd(q, k, v, o, lse, do.view(B, S, H, hd) if do.is_contiguous() else do.reshape(B, S, H, hd), window, sinks, hd ** -0.5,
+                    out=(dq, dk, dv))
+        _rotate(dq, dk, positions, freqs, half, magnitude, True, dq, dk)
+        return (dqkv,) + (None,) * 9
+
+
+def rotary_window_attention_packed(qkv, positions, freqs, heads, kv_heads, layout, magnitude, window, sinks):
+    """Kernel front-end of ``ops.functional.rotary_window_attention``."""
+    hd = qkv.shape[2] // (heads + 2 * kv_heads)
+    return _RotaryWindowPackedFn.apply(qkv, positions, freqs, layout == "half", float(magnitude), heads, kv_heads, hd, window, sinks)

@@ -30,6 +30,11 @@ def set_activation_recompute(on: bool) -> bool:
     return old
 
 
+def activation_recompute() -> bool:
+    """Whether outputs are tagged."""
+    return _RECOMPUTE
+
+
 def _tag(out: torch.Tensor, kind: str, *srcs):
     if _RECOMPUTE and torch.is_grad_enabled():
         out._rtp_recompute = (kind, srcs)
@@ -348,6 +353,26 @@ def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
     if R.kernel_takes(q) and get_backend() != "functional":
         return R.rotary(q, k, positions, freqs, layout, magnitude)
     return R.rotary_plain(q, k, positions, freqs, layout, magnitude)
+
+
+def rotary_window_attention(qkv, positions, freqs, heads, kv_heads=None, layout="half", magnitude=1.0, window=None, sinks=0):
+    """Rotary positions and causal attention of a packed projection ``qkv`` [B, S, (heads + 2 * kv_heads) * hd], whose columns are the
+    heads of q, then those of k, then those of v -> [B, S, heads * hd].  ``window`` / ``sinks`` as in :func:`window_attention` (None:
+    every earlier token is seen); the other arguments as in :func:`rotary`."""
+    from . import flash, rotary as R
+    kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
+        raise ValueError(f"rotary_window_attention: qkv must be [B, S, (heads + 2 * kv_heads) * hd], got {tuple(qkv.shape)} for {heads} and {kv_heads} heads")
+    B, S, W = qkv.shape
+    hd = W // (heads + 2 * kv_heads)
+    window = max(S, 1) if window is None else window
+    q, k, v = qkv.view(B, S, heads + 2 * kv_heads, hd).split((heads, kv_heads, kv_heads), dim=2)
+    R.check_args(q, k, positions, freqs, layout)
+    flash.check_window_args(q, k, v, window, sinks)
+    if use_kernels(qkv) and hd in (64, 128) and qkv.numel() and qkv.is_contiguous() and qkv.data_ptr() % 16 == 0:
+        return flash.rotary_window_attention_packed(qkv, positions, freqs, heads, kv_heads, layout, magnitude, window, sinks)
+    q, k = rotary(q, k, positions, freqs, layout, magnitude)
+    return window_attention(q, k, v, window, sinks).reshape(B, S, heads * hd)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

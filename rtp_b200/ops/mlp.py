@@ -2,8 +2,8 @@
 
 Forward is two launches: both projections with the activation and the product in their epilogue, then the down projection.  Backward is
 two as well: ``dy Wd``, whose epilogue turns the product's gradient into those of gate and up and makes the product again, then both
-weight gradients and the input gradient side by side.  Products of few rows fall into slices of their contraction, which one more
-launch adds up."""
+weight gradients and the input gradient side by side.  Products of few rows, and small weight gradients over many, fall into slices
+of their contraction, which one more launch each adds up."""
 import ctypes as C
 
 import torch
@@ -15,7 +15,7 @@ class GatedFwd(C.Structure):
     _fields_ = [
         ("T", C.c_int), ("D", C.c_int), ("F", C.c_int), ("O", C.c_int),
         ("x", C.c_void_p), ("ldx", C.c_longlong), ("w_gu", C.c_void_p), ("ld_gu", C.c_longlong),
-        ("w_d", C.c_void_p), ("ld_d", C.c_longlong), ("gu", C.c_void_p), ("h", C.c_void_p), ("y", C.c_void_p),
+        ("w_d", C.c_void_p), ("ld_d", C.c_longlong), ("gu", C.c_void_p), ("h", C.c_void_p), ("y", C.c_void_p), ("whole", C.c_int),
         ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
     ]
 
@@ -26,7 +26,7 @@ class GatedBwd(C.Structure):
         ("x", C.c_void_p), ("ldx", C.c_longlong), ("dy", C.c_void_p), ("ldy", C.c_longlong),
         ("w_gu", C.c_void_p), ("ld_gu", C.c_longlong), ("w_d", C.c_void_p), ("ld_d", C.c_longlong),
         ("gu", C.c_void_p), ("dgu", C.c_void_p), ("h", C.c_void_p), ("dx", C.c_void_p), ("dw_gu", C.c_void_p), ("dw_d", C.c_void_p),
-        ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
+        ("whole", C.c_int), ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
     ]
 
 
@@ -85,60 +85,62 @@ def _check(rc, what, launches):
     _lib.launches += launches - 1
 
 
-def gated_fwd(x, w_gu, w_d, keep):
-    """(y, gate | up or None) of [T, D] rows."""
+def gated_fwd(x, w_gu, w_d, keep, whole=False):
+    """(y, gate | up or None) of [T, D] rows.  ``whole``: sums in the order of separate layers."""
     if x.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(x.device):
-            return gated_fwd(x, w_gu, w_d, keep)
+            return gated_fwd(x, w_gu, w_d, keep, whole)
     T, D = x.shape
     O, F = w_d.shape
     h, y = x.new_empty(T, F), x.new_empty(T, O)
     gu = x.new_empty(T, 2 * F) if keep else None
     a = GatedFwd(T, D, F, O, x.data_ptr(), x.stride(0), w_gu.data_ptr(), w_gu.stride(0), w_d.data_ptr(), w_d.stride(0),
-                 gu.data_ptr() if keep else None, h.data_ptr(), y.data_ptr(), _lib.status_word(x.device).data_ptr(), None, 0)
+                 gu.data_ptr() if keep else None, h.data_ptr(), y.data_ptr(), whole, _lib.status_word(x.device).data_ptr(), None, 0)
     L = _L()
     s = _scratch(L, "fwd", a, x.device)
     _check(L.rtp_gated_fwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_fwd", 2 if s is None else 3)
     return y, gu
 
 
-def gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d):
+def gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d, whole=False):
     """Fills those of dx [T, D], dw_gu [2 * F, D] and dw_d [O, F] (dense) that are not None."""
     if x.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(x.device):
-            return gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d)
+            return gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d, whole)
     T, D = x.shape
     O, F = w_d.shape
     dgu = torch.empty_like(gu)
     h = x.new_empty(T, F) if dw_d is not None else None
     p = [t.data_ptr() if t is not None else None for t in (h, dx, dw_gu, dw_d)]
     a = GatedBwd(T, D, F, O, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), w_gu.data_ptr(), w_gu.stride(0), w_d.data_ptr(),
-                 w_d.stride(0), gu.data_ptr(), dgu.data_ptr(), *p, _lib.status_word(x.device).data_ptr(), None, 0)
+                 w_d.stride(0), gu.data_ptr(), dgu.data_ptr(), *p, whole, _lib.status_word(x.device).data_ptr(), None, 0)
     L = _L()
     s = _scratch(L, "bwd", a, x.device)
     _check(L.rtp_gated_bwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_bwd", 2 if s is None else 3)
 
 
 class _GatedMlpFn(torch.autograd.Function):
-    """``owners``: None, or the two rotated modules of one rank whose flat shards the weights are; their gradients then come as flat
-    buffers.  ``rebuild``: (kind, sources) of an input that can be made again (see ``ops.functional``), which is then not kept."""
+    """``owners``: None, or the two rotated modules of one rank whose flat shards the weights are; backward then reads the weights where
+    they are, as that of a rotated layer does, and their gradients come as flat buffers.  ``rebuild``: (kind, sources) of an
+    input that can be made again (see ``ops.functional``), which is then not kept."""
 
     @staticmethod
     def forward(ctx, x, w_gu, w_d, owners, rebuild, needs_bwd):
         x2, wg, wd = _rows(x.reshape(-1, x.shape[-1])), _rows(w_gu), _rows(w_d)
-        y, gu = gated_fwd(x2, wg, wd, needs_bwd)
+        y, gu = gated_fwd(x2, wg, wd, needs_bwd, owners is not None)
         if needs_bwd:
             kind, srcs = rebuild if rebuild is not None else (None, (x2,))
             ctx.kind, ctx.tensors = kind, [torch.is_tensor(s) for s in srcs]
             ctx.consts = [s for s in srcs if not torch.is_tensor(s)]
-            ctx.save_for_backward(wg, wd, gu, *[s for s in srcs if torch.is_tensor(s)])
+            ctx.save_for_backward(gu, *(() if owners else (wg, wd)), *[s for s in srcs if torch.is_tensor(s)])
             ctx.owners, ctx.shape = owners, x.shape
         return y.view(*x.shape[:-1], w_d.shape[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        wg, wd, gu, *kept = ctx.saved_tensors
+        gu, *kept = ctx.saved_tensors
+        wg, wd = [_rows(o.linear.weight) for o in ctx.owners] if ctx.owners else (kept.pop(0), kept.pop(0))
         if ctx.kind is None:
             x2 = kept[0]
         else:
@@ -152,7 +154,7 @@ class _GatedMlpFn(torch.autograd.Function):
         grads = [None if not n else w.new_empty(w.shape) if f is None else f[:w.numel()].view(w.shape)
                  for w, f, n in zip((wg, wd), flats, ctx.needs_input_grad[1:3])]
         dx = x2.new_empty(x2.shape) if ctx.needs_input_grad[0] else None
-        gated_bwd(x2, dy2, wg, wd, gu, dx, *grads)
+        gated_bwd(x2, dy2, wg, wd, gu, dx, *grads, ctx.owners is not None)
         for o, f in zip(ctx.owners or (), flats):
             if f is not None:
                 o._last_flat_grad = f
@@ -165,8 +167,9 @@ def gated_mlp(x, w_gate_up, w_down, owners=None):
     if not kernel_takes(x, w_gate_up, w_down):
         raise ValueError(f"gated_mlp: the kernels take bf16 CUDA tensors with sizes that are multiples of 8, got {x.dtype} {tuple(x.shape)} on {x.device}")
     needs_bwd = torch.is_grad_enabled() and (x.requires_grad or w_gate_up.requires_grad or w_down.requires_grad)
-    rebuild = getattr(x, "_rtp_recompute", None) if needs_bwd else None
+    # an input changed in place since its producer tagged it is kept
+    rebuild = getattr(x, "_rtp_recompute", None) if needs_bwd and x._version == 0 else None
     if not needs_bwd:
         x2 = _rows(x.reshape(-1, x.shape[-1]))
-        return gated_fwd(x2, _rows(w_gate_up), _rows(w_down), False)[0].view(*x.shape[:-1], w_down.shape[0])
+        return gated_fwd(x2, _rows(w_gate_up), _rows(w_down), False, owners is not None)[0].view(*x.shape[:-1], w_down.shape[0])
     return _GatedMlpFn.apply(x, w_gate_up, w_down, owners, rebuild, needs_bwd)

@@ -21,6 +21,8 @@ class RotaryArgs(C.Structure):
         ("q", C.c_void_p), ("k", C.c_void_p), ("qo", C.c_void_p), ("ko", C.c_void_p),
         ("q_sb", C.c_longlong), ("q_ss", C.c_longlong), ("q_sh", C.c_longlong),
         ("k_sb", C.c_longlong), ("k_ss", C.c_longlong), ("k_sh", C.c_longlong),
+        ("qo_sb", C.c_longlong), ("qo_ss", C.c_longlong), ("qo_sh", C.c_longlong),
+        ("ko_sb", C.c_longlong), ("ko_ss", C.c_longlong), ("ko_sh", C.c_longlong),
         ("positions", C.c_void_p), ("pos_sb", C.c_longlong), ("pos_ss", C.c_longlong),
         ("freqs", C.c_void_p), ("magnitude", C.c_float),
         ("pos64", C.c_int), ("B", C.c_int), ("S", C.c_int), ("q_heads", C.c_int), ("k_heads", C.c_int), ("hd", C.c_int),
@@ -60,7 +62,7 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling="none", factor=1.0, or
         raise ValueError("theta, factor and original_length must be positive")
     if scaling == "ntk" and rotary_dim > 2:
         theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
-    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
@@ -69,7 +71,7 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling="none", factor=1.0, or
         turns = original_length * f / (2 * math.pi)
         keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
         f = f * keep + f / factor * (1.0 - keep)
-    return f.to(device) if device is not None else f
+    return f
 
 
 def rotary_magnitude(scaling="none", factor=1.0):
@@ -105,30 +107,34 @@ def kernel_takes(q):
     return q.is_cuda and q.dtype in _TYPES and q.shape[3] <= 256 and q.shape[3] % 2 == 0
 
 
-def _side(t):
-    """(tensor, its output, addresses, strides) of q or k; strides of a single batch entry, position or head do not matter."""
+def _side(t, o):
+    """(tensor, its output, addresses, strides in and out, heads) of q or k; strides of a single batch entry, position or head do not
+    matter.  ``o``: where to (None: a new contiguous tensor)."""
     if t is None:
-        return None, None, None, None, 0, 0, 0, 0
-    (B, S, H, _), (sb, ss, sh, sd) = t.shape, t.stride()
-    if sd != 1:
+        return None, None, None, None, (0, 0, 0), (0, 0, 0), 0
+    if t.stride(3) != 1:
         t = t.contiguous()
-        sb, ss, sh, _ = t.stride()
-    o = torch.empty_like(t, memory_format=torch.contiguous_format)
-    return t, o, t.data_ptr(), o.data_ptr(), sb if B > 1 else 0, ss if S > 1 else 0, sh if H > 1 else 0, H
+    if o is None:
+        o = torch.empty_like(t, memory_format=torch.contiguous_format)
+    B, S, H, _ = t.shape
+    a, b = t.stride(), o.stride()
+    if B == 1 or S == 1 or H == 1:
+        a, b = ([s if n > 1 else 0 for s, n in zip(st, t.shape)] for st in (a, b))
+    return t, o, t.data_ptr(), o.data_ptr(), a[:3], b[:3], H
 
 
-def _rotate(q, k, positions, freqs, half, magnitude, backward):
-    """One launch for q and / or k (either may be None)."""
+def _rotate(q, k, positions, freqs, half, magnitude, backward, qo=None, ko=None):
+    """One launch for q and / or k (either may be None), into new tensors or qo and ko (which may be q and k)."""
     one = q if q is not None else k
     if one.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(one.device):
-            return _rotate(q, k, positions, freqs, half, magnitude, backward)
+            return _rotate(q, k, positions, freqs, half, magnitude, backward, qo, ko)
     B, S, _, hd = one.shape
-    q, qo, qp, qop, qb, qs, qh, H = _side(q)          # copies live until the launch
-    k, ko, kp, kop, kb, ks, kh, Hk = _side(k)
+    q, qo, qp, qop, qs, qos, H = _side(q, qo)         # copies live until the launch
+    k, ko, kp, kop, ks, kos, Hk = _side(k, ko)
     freqs = freqs.contiguous()
     st = positions.stride()
-    a = RotaryArgs(qp, kp, qop, kop, qb, qs, qh, kb, ks, kh, positions.data_ptr(), st[0] if len(st) == 2 and positions.shape[0] > 1 else 0,
+    a = RotaryArgs(qp, kp, qop, kop, *qs, *ks, *qos, *kos, positions.data_ptr(), st[0] if len(st) == 2 and positions.shape[0] > 1 else 0,
                    st[-1], freqs.data_ptr(), magnitude, positions.dtype == torch.int64, B, S, H, Hk, hd, 2 * freqs.shape[0], half,
                    _TYPES[one.dtype], backward)
     L = _L()

@@ -248,3 +248,30 @@ def test_refusals_on_the_gpu():
     with pytest.raises(RuntimeError):
         g = torch.autograd.grad(FO.gated_mlp(x.requires_grad_(), wgu, wd).sum(), x, create_graph=True)[0]
         g.sum().backward()
+
+
+@pytest.mark.parametrize("T,D,n", [(8192, 64, 64), (8200, 128, 200), (9000, 256, 264), (8191, 64, 64)])
+def test_small_weights_over_many_rows(T, D, n):
+    """Their gradients fall into slices from 8192 rows on."""
+    import ctypes as C
+    both = mlp.GatedBwd(T=T, D=D, F=n, O=D, dw_gu=1, dw_d=1)
+    assert (mlp._L().rtp_gated_bwd_scratch(C.byref(both)) > 0) == (T >= 8192)
+    check(*tensors(T, D, n, D, n))
+
+
+@pytest.mark.parametrize("T,D,n", [(8, 2048, 8192), (300, 256, 1000), (9000, 128, 264), (1000, 512, 1024)])
+def test_layers_give_the_same_bits(T, D, n):
+    """A packed projection, the activation and a down projection as rotated layers of one rank, fused and one by one."""
+    from rtp_b200.module.linear import ColumnParallelLinear, RowParallelLinear
+    from rtp_b200.parallel import engine, fused
+    torch.manual_seed(T)
+    kw = dict(bias=False, device="cuda", dtype=torch.bfloat16)
+    up, down = ColumnParallelLinear(D, 2 * n, packed_parts=2, **kw), RowParallelLinear(n, D, **kw)
+    x, _, _, dy = tensors(T, D, 8, D)
+    leaves = [x.requires_grad_(), up.linear.weight, down.linear.weight]
+    y = fused.gated_mlp(up, down, x)
+    got = [y, *torch.autograd.grad(y, leaves, dy)]
+    y = down(FO.swiglu_packed(up(x)))
+    want = [y, *torch.autograd.grad(y, leaves, dy)]
+    engine.check_all()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
