@@ -417,6 +417,15 @@ __device__ __forceinline__ void umma_rows(uint32_t d, uint32_t a_tmem, uint32_t 
                  (add || kk > 0) ? 1u : 0u);
 }
 
+// The same in two halves, of which the second waits: `half` h takes the h-th 32 of the 64 rows of B that go with each half of A.
+__device__ __forceinline__ void umma_half_rows(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, int half, bool add) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kk = (i >> 1) * 4 + half * 2 + (i & 1);
+    umma_bf16_ts(d, a_tmem + (kk >> 2) * 64 + (kk & 3) * 8, make_smem_desc(b + kk * 2048, kSub, 1024), idesc, (add || half || i > 0) ? 1u : 0u);
+  }
+}
+
 // =====================================================================================================  window
 // The key blocks that a tile of 128 queries works on: those of its window from block `lo` on, and the `ns` first ones, which hold the
 // sinks (0 where the window reaches into them: then `lo` is 0).  Step i takes block at(i): the first of the window, the sinks, the
@@ -571,7 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, false)) {
         const FwdWork w = n == 0 ? first : fwd_work<WIN>(p, blk);
         const int b = w.b, h = w.h;
-        const int cq = head_col(p.q, h), ck = head_col(p.k, h), cv = head_col(p.v, h);
+        const int hk = WIN ? p.by_qpk(h) : h;
+        const int cq = head_col(p.q, h), ck = head_col(p.k, hk), cv = head_col(p.v, hk);
         auto load_q = [&](int t) {
           const uint32_t ph = nq[t]++ & 1u;
           if (!wait(F_QEMPTY + t, ph ^ 1u)) return false;
@@ -919,7 +929,7 @@ __global__ void __launch_bounds__(256) flash_delta_kernel(DRef o, DRef g, float*
 // Barriers: tile t full t, empty 7 + t; the statistics of a block of queries (-log-sum-exp, -delta: the producer warp) beside
 // its Q tile; accumulators complete, and read out.
 enum { B_FULL = 0, B_EMPTY = 7, B_STAT = 14 /* 2 */, B_SFULL = 16 /* 2 */, B_PFULL = 18, B_DPFULL = 19, B_DSFULL = 20, B_ACC = 21,
-       B_ACCREAD = 22, B_WFULL = 23, B_TAKEN = 24, B_DRAIN = 25 };
+       B_ACCREAD = 22, B_WFULL = 23, B_TAKEN = 24, B_DRAIN = 25, B_PTAIL = 26, B_DSTAIL = 27 };
 
 // What blockIdx.x stands for: the key block kb, or (kb < 0) the query block qb, of head h of batch entry b.
 struct BwdWork {
@@ -1019,10 +1029,10 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
   const int nqb = (M.Sq + kBlk - 1) / kBlk, nkb = (M.Sk + kBlk - 1) / kBlk;
   // counts by barrier index: copies and commits 1; statistics 32 (lanes); P and dS, accumulators read 8 (one per row warp); next work
   // 1 and 10 (producer, issuer, eight row warps)
-  const int counts[26] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 32, 32, 1, 1, 8, 1, 8, 1, 8, 1, 10, 1};
+  const int counts[28] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 32, 32, 1, 1, 8, 1, 8, 1, 8, 1, 10, 1, 8, 8};
   const BwdWork first = bwd_work<WIN>(p, (int)blockIdx.x);       // before the wait for the previous kernel, as in forward
   asm volatile("" ::"r"(first.b), "r"(first.h), "r"(first.kb), "r"(first.qb));
-  const uint32_t tmem = setup_cta(ctl, counts, 26, warp, lane);
+  const uint32_t tmem = setup_cta(ctl, counts, 28, warp, lane);
   volatile uint32_t* abort_flag = &ctl->abort_flag;
   unsigned long long* status = p.status;
   const unsigned long long tmo = p.timeout_ns;
@@ -1053,7 +1063,8 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
     for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, true)) {
       const BwdWork w = n == 0 ? first : bwd_work<WIN>(p, blk);
       const int b = w.b, h = w.h;
-      const int cq = head_col(p.q, h), ck = head_col(p.k, h), cv = head_col(p.v, h), cg = head_col(p.dout, h);
+      const int hk = WIN ? p.by_qpk(h) : h;
+      const int cq = head_col(p.q, h), ck = head_col(p.k, hk), cv = head_col(p.v, hk), cg = head_col(p.dout, h);
       if (w.kb >= 0) {
         const int i0 = WIN ? w.s0 : M.causal ? w.kb : 0, i1 = WIN ? w.s0 + w.n : nqb;
         ok = load(0, &p.mk, p.k_seq1, ck, b, w.kb * kBlk);
@@ -1120,6 +1131,21 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
         issued = true;
         return true;
       };
+      // an accumulator += P or dS (from `a_tmem`) x tile bt, as soon as the rows have made it (window: each half of it)
+      // In halves, the first product runs under the second half's exponentials: 2 to 3 % of the backward.
+      auto rows = [&](int full, int tail, uint32_t ph, uint32_t d, uint32_t a_tmem, int bt, bool add) {
+        if (!wait(full, ph)) return false;
+        tc_fence_after();
+        if constexpr (WIN) {
+          umma_half_rows(d, a_tmem, at(bt), id_t, 0, add);
+          if (!wait(tail, ph)) return false;
+          tc_fence_after();
+          umma_half_rows(d, a_tmem, at(bt), id_t, 1, add);
+        } else {
+          umma_rows(d, a_tmem, at(bt), id_t, add);
+        }
+        return true;
+      };
       for (int blk = (int)blockIdx.x; blk >= 0 && ok; blk = following(n++, false)) {
         const BwdWork w = n == 0 ? first : bwd_work<WIN>(p, blk);
         mbar_arrive(&bar[B_TAKEN]);
@@ -1131,14 +1157,10 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           for (int it = 0; it < nit && ok; ++it) {
             const int st = it & 1, ot = st ^ 1;
             const bool more = it + 1 < nit, end = it + 2 == nit;
-            if (!wait(B_PFULL, np++ & 1u)) { ok = false; break; }
-            tc_fence_after();
-            umma_rows(tAcc, tS, at(4 + st), id_t, it > 0);
+            if (!rows(B_PFULL, B_PTAIL, np++ & 1u, tAcc, tS, 4 + st, it > 0)) { ok = false; break; }
             done_with(4 + st);
             if (more && !product(tS, 0, 2 + ot, B_SFULL, end, false)) { ok = false; break; }
-            if (!wait(B_DSFULL, nds++ & 1u)) { ok = false; break; }
-            tc_fence_after();
-            umma_rows(tAcc + HD, tP, at(2 + st), id_t, it > 0);
+            if (!rows(B_DSFULL, B_DSTAIL, nds++ & 1u, tAcc + HD, tP, 2 + st, it > 0)) { ok = false; break; }
             if constexpr (ONE) {                         // dQ from dS^T in shared memory, into the columns of S
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
@@ -1157,9 +1179,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           auto issue_dp = [&](int j) { return product(tP, 1, 5 + (j & 1), B_DPFULL, j + 1 == nb, true); };
           ok = tile(0) && issue_s(0) && tile(1) && issue_dp(0) && wait(B_ACCREAD, read) && (nb < 2 || issue_s(1));
           for (int j = 0; j < nb && ok; ++j) {
-            if (!wait(B_DSFULL, nds++ & 1u)) { ok = false; break; }
-            tc_fence_after();
-            umma_rows(tAcc, tP, at(2 + j % 3), id_t, j > 0);
+            if (!rows(B_DSFULL, B_DSTAIL, nds++ & 1u, tAcc, tP, 2 + j % 3, j > 0)) { ok = false; break; }
             done_with(2 + j % 3);
             if (j + 1 == nb) umma_commit(&bar[B_ACC]);
             else ok = issue_dp(j + 1) && (j + 2 >= nb || issue_s(j + 2));
@@ -1236,22 +1256,18 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           tmem_ld32f(aS, x);
           tmem_ld32f(aS + 32, x + 32);
           tmem_ld_wait();
-          if (keys_plain && (WIN ? all_seen(M, qb * kBlk, k0) : !(M.causal && it == 0))) {      // the diagonal crosses a causal key block's first query block
+          if (WIN || (keys_plain && !(M.causal && it == 0))) {   // the diagonal crosses a causal key block's first query block
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
               const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, make_float2(nl[i], nl[i + 1]));
               x[i] = u.x; x[i + 1] = u.y;
             }
-          } else if constexpr (WIN) {
-            // the queries that see the key: from its own position to the end of the window, a sink to the last
-            const int lo = key - M.ahead - qbase, hi = key_dead ? lo : key < M.sinks ? 64 : lo + M.window;
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              const float2 u = fma2(make_float2(x[i], x[i + 1]), sc, make_float2(nl[i], nl[i + 1]));
-              x[i] = u.x; x[i + 1] = u.y;
+            if (WIN && !(keys_plain && all_seen(M, qb * kBlk, k0))) {
+              // the queries that see the key: from its own position to the end of the window, a sink to the last
+              const int lo = key - M.ahead - qbase, hi = key_dead ? lo : key < M.sinks ? 64 : lo + M.window;
+              keep_seen(x, below(hi) & ~below(lo));
+              keep_seen(x + 32, below(hi - 32) & ~below(lo - 32));
             }
-            keep_seen(x, below(hi) & ~below(lo));
-            keep_seen(x + 32, below(hi - 32) & ~below(lo - 32));
           } else {
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
@@ -1280,8 +1296,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
             } else {
               store_bf16x32(aS + (uint32_t)(c * 16), e);
             }
+            if (WIN && c == 0) publish_rows(&bar[B_PFULL], lane);
           }
-          publish_rows(&bar[B_PFULL], lane);
+          publish_rows(&bar[WIN ? B_PTAIL : B_PFULL], lane);
           if (tr && it < 16) tr[it * 8 + 2] = clock64();
           if (!wait(B_DPFULL, ndp++ & 1u)) { ok = false; break; }
           tc_fence_after();
@@ -1312,9 +1329,10 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
                     make_uint4(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7]));
               }
             }
+            if (WIN && c == 0) publish_rows(&bar[B_DSFULL], lane);
           }
           if constexpr (ONE) fence_proxy_async_smem();
-          publish_rows(&bar[B_DSFULL], lane);
+          publish_rows(&bar[WIN ? B_DSTAIL : B_DSFULL], lane);
           if (tr && it < 16) tr[it * 8 + 4] = clock64();
         }
       } else {
@@ -1378,47 +1396,56 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
               x[i] = u.x; x[i + 1] = u.y;
             }
             store_bf16x32(aP + (uint32_t)(c * 16), x + 32 * c);
+            if (WIN && c == 0) publish_rows(&bar[B_DSFULL], lane);
           }
-          publish_rows(&bar[B_DSFULL], lane);
+          publish_rows(&bar[WIN ? B_DSTAIL : B_DSFULL], lane);
+        }
+      }
+      const int r0 = (w.kb >= 0 ? w.kb : w.qb) * kBlk + (warp & 3) * 32;      // the warp's first row
+      // window: where the results go, looked up under the last product
+      [[maybe_unused]] __nv_bfloat16 *dst0 = nullptr, *dst1 = nullptr;
+      [[maybe_unused]] long long pitch0 = 0, pitch1 = 0;
+      if constexpr (WIN) {
+        if (w.kb < 0) {
+          dst0 = row_ptr(p.dq, b, r0, h) + wg * (HD / 2);
+          pitch0 = p.dq.ss;
+        } else {
+          const int hk = p.by_qpk(h);
+          dst0 = row_ptr(p.dv, b, r0, hk) + wg * (HD / 2);
+          dst1 = row_ptr(p.dk, b, r0, hk) + wg * (HD / 2);
+          pitch0 = p.dv.ss;
+          pitch1 = p.dk.ss;
         }
       }
       if (ok) ok = wait(B_ACC, n & 1u);
       if (!ok) break;
       tc_fence_after();
-      const int r0 = (w.kb >= 0 ? w.kb : w.qb) * kBlk + (warp & 3) * 32;      // the warp's first row
       const int nacc = ONE ? 3 : w.kb >= 0 ? 2 : 1;
-      if constexpr (WIN) {               // everything at once: one wait, and the accumulators are free for the next piece
-        float o[HD];                     // dV and dK, half a row each, or that of dQ
+      if constexpr (WIN) {
+        // 32 columns at a time, one after the other: with all of them read at once, unrolled, the steps before spilled and their code had
+        // to be fetched again (backward of 32768 x 16 heads, window 2048, 2 150 -> 1 920 us, 4 x 2048 x 16, window 512, 223 -> 188)
         const bool is_q = w.kb < 0;
+        const int chunks = is_q ? HD / 64 : HD / 32;
+#pragma unroll 1
+        for (int ch = 0; ch < chunks; ++ch) {
+          const int a = ch / (HD / 64), c = ch % (HD / 64);
+          float o[32];
+          tmem_ld32f(tAcc + (uint32_t)(a * HD) + lane_off + (uint32_t)(wg * (HD / 2) + c * 32), o);
+          tmem_ld_wait();
+          if (ch + 1 == chunks) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar[B_ACCREAD]);
+          }
+          const float mul = a || is_q ? M.sm_scale : 1.f;
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+          for (int i = 0; i < 32; ++i) o[i] *= mul;
+          if (w.piece >= 0) {            // [piece][dV, dK][HD / 4][key][4]: the lanes of a store side by side
+            float4* sum = reinterpret_cast<float4*>(p.part) + ((long long)w.piece * 2 * (HD / 4) + a * (HD / 4) + wg * (HD / 8) + c * 8) * kBlk + rt;
 #pragma unroll
-          for (int c = 0; c < HD / 64; ++c)
-            if (a == 0 || !is_q) tmem_ld32f(tAcc + (uint32_t)(a * HD) + lane_off + (uint32_t)(wg * (HD / 2) + c * 32), o + a * (HD / 2) + c * 32);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar[B_ACCREAD]);
-        const float mul0 = is_q ? M.sm_scale : 1.f;
-#pragma unroll
-        for (int i = 0; i < HD / 2; ++i) { o[i] *= mul0; o[HD / 2 + i] *= M.sm_scale; }
-        if (w.piece >= 0) {              // [piece][dV, dK][HD / 4][key][4]: the lanes of a store side by side
-          float4* sum = reinterpret_cast<float4*>(p.part) + (long long)w.piece * 2 * (HD / 4) * kBlk + wg * (HD / 8) * kBlk + rt;
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i) {
-              const float* e = o + a * (HD / 2) + 4 * i;
-              sum[(a * (HD / 4) + i) * kBlk] = make_float4(e[0], e[1], e[2], e[3]);
-            }
-        } else {
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            if (a && is_q) break;
-            const DRef& out = is_q ? p.dq : a ? p.dk : p.dv;
-            __nv_bfloat16* dst = row_ptr(out, b, r0, is_q ? h : p.by_qpk(h)) + wg * (HD / 2);
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c) store_rows32(dst + c * 32, out.ss, (is_q ? M.Sq : M.Sk) - r0, o + a * (HD / 2) + c * 32, lane);
+            for (int i = 0; i < 8; ++i) sum[i * kBlk] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else {
+            store_rows32((a ? dst1 : dst0) + c * 32, a ? pitch1 : pitch0, (is_q ? M.Sq : M.Sk) - r0, o, lane);
           }
         }
       } else

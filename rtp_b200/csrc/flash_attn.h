@@ -40,8 +40,8 @@ typedef struct {
 } RtpFlashArgs;
 
 // Causal attention over a window of keys and the first few (sinks): query i stands at position p = i + Sk - Sq and sees key j if
-// j <= p and (j > p - window or j < sinks).  H query heads share kv_heads key and value heads: head h reads k and v at
-// its col(h), which a group of neighbours has in common (hpg = H / kv_heads, hstride = 0); dk and dv have kv_heads heads.
+// j <= p and (j > p - window or j < sinks).  H query heads share kv_heads key and value heads: head h reads
+// head h / (H / kv_heads) of k and v, which have kv_heads heads, as dk and dv.
 // f.causal, f.mask, f.kpm and f.drop_p are zero.  f.lse may be null in a forward without a backward.
 typedef struct {
   RtpFlashArgs f;

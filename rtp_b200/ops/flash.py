@@ -258,19 +258,12 @@ def _addressable(t):
     return t.clone(memory_format=torch.contiguous_format)      # also of a contiguous tensor at an odd address
 
 
-def _shared_ref(t, group):
-    """FlashRef of a [B, S, Hk, hd] view whose heads serve ``group`` query heads each."""
-    _, _, H, hd = t.shape
-    sb, ss, sh, _ = t.stride()
-    return _lib.FlashRef(t.data_ptr(), sb, ss, (H - 1) * sh + hd, 0, group, sh, 0)
-
-
 def _window_args(q, k, v, o, lse, window, sinks, sm_scale):
     B, Sq, H, hd = q.shape
     Sk, Hk = k.shape[1:3]
     a = _lib.WindowArgs()
     f, most = a.f, 2 ** 31 - 1
-    f.q, f.o, f.k, f.v = _ref4(q), _ref4(o), _shared_ref(k, H // Hk), _shared_ref(v, H // Hk)
+    f.q, f.o, f.k, f.v = _ref4(q), _ref4(o), _ref4(k), _ref4(v)
     f.lse = lse.data_ptr() if lse is not None else None
     f.B, f.H, f.Sq, f.Sk, f.head_dim, f.sm_scale = B, H, Sq, Sk, hd, sm_scale
     f.status = _lib.status_word(q.device).data_ptr()
@@ -314,7 +307,7 @@ def _window_bwd(q, k, v, o, lse, do, window, sinks, sm_scale, out=None):
     delta = torch.empty_like(lse)
     a = _window_args(q, k, v, o, lse, window, sinks, sm_scale)
     f = a.f
-    f.dout, f.dq, f.dk, f.dv, f.delta = _ref4(do), _ref4(dq), _shared_ref(dk, 1), _shared_ref(dv, 1), delta.data_ptr()
+    f.dout, f.dq, f.dk, f.dv, f.delta = _ref4(do), _ref4(dq), _ref4(dk), _ref4(dv), delta.data_ptr()
     L = _lib.lib()
     need = L.rtp_window_bwd_scratch(C.byref(a))
     if need:
