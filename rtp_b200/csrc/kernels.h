@@ -78,12 +78,12 @@ int rtp_top2_gate_bwd(const float* gates, const int* idx, const unsigned char* v
                       const float* d_gate_w, const float* d_l_aux, float* dlogits, int S, int E, void* stream);
 int rtp_rope(const void* x, void* y, const float* cosv, const float* sinv, long long T, int H, int hd, int S, int inner,
              int backward, void* stream);
-// Rotary positions of q and k (rotary.cu): views [B, S, heads, hd] with unit stride inside a head (strides in elements), in and out, which
-// may be the same; k_heads = 0: q alone.  Pair i of the first `rot` elements turns by positions[b, s] * freqs[i] radians.
+// Rotary positions of q and k (rotary.cu): views [B, S, heads, hd] with unit stride inside a head (strides in elements; of a
+// single batch entry, position or head any), in and out, which may be the same; k_heads = 0: q alone.  Pair i of the first `rot` elements turns by positions[b, s] * freqs[i] radians.
 typedef struct {
   const void *q, *k;
   void *qo, *ko;
-  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, qo_sb, qo_ss, qo_sh, ko_sb, ko_ss, ko_sh;
+  long long q_st[4], k_st[4], qo_st[4], ko_st[4];      // of batch, position, head and element (1)
   const void* positions;               // int64 (pos64 = 1) or int32 at b * pos_sb + s * pos_ss
   long long pos_sb, pos_ss;
   const double* freqs;                 // [rot / 2]

@@ -141,17 +141,20 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
 }
 
+// q or k as the kernel sees it: strides of a single batch entry, position or head do not matter.
+Side side(const RtpRotary& a, const void* in, void* out, const long long* st, const long long* ost, int heads) {
+  const bool b = a.B > 1, s = a.S > 1, h = heads > 1;
+  return Side{in, out, b ? st[0] : 0, s ? st[1] : 0, h ? st[2] : 0, b ? ost[0] : 0, s ? ost[1] : 0, h ? ost[2] : 0, heads};
+}
 // The widest access (bytes) that pairs, tail, strides and addresses allow.
-int access_bytes(const RtpRotary& a, int size) {
+int access_bytes(const RtpRotary& a, const Side& q, const Side& k, int size) {
   for (int bytes = 16; bytes > size; bytes >>= 1) {
     const int v = bytes / size;
-    auto fits = [&](const void* x, long long sb, long long ss, long long sh) {
-      return (reinterpret_cast<uintptr_t>(x) & (uintptr_t)(bytes - 1)) == 0 && sb % v == 0 && ss % v == 0 && sh % v == 0;
+    auto fits = [&](const Side& x) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(x.in) | reinterpret_cast<uintptr_t>(x.out);
+      return !x.heads || (at % bytes == 0 && (x.sb | x.ss | x.sh | x.osb | x.oss | x.osh) % v == 0);
     };
-    if (a.hd % v || (a.half_layout ? a.rot / 2 : a.rot) % v) continue;
-    if (a.q_heads && (!fits(a.q, a.q_sb, a.q_ss, a.q_sh) || !fits(a.qo, a.qo_sb, a.qo_ss, a.qo_sh))) continue;
-    if (a.k_heads && (!fits(a.k, a.k_sb, a.k_ss, a.k_sh) || !fits(a.ko, a.ko_sb, a.ko_ss, a.ko_sh))) continue;
-    return bytes;
+    if (a.hd % v == 0 && (a.half_layout ? a.rot / 2 : a.rot) % v == 0 && fits(q) && fits(k)) return bytes;
   }
   return size;
 }
@@ -175,10 +178,10 @@ int rtp_rotary(const RtpRotary* a, void* stream) {
   const long long tokens = (long long)a->B * a->S;
   const int heads = a->q_heads + a->k_heads;
   if (!tokens || !heads) return 0;
-  const int size = a->dtype == 2 ? 4 : 2, bytes = access_bytes(*a, size), v = bytes / size;
   Params P = {};
-  P.q = Side{a->q, a->qo, a->q_sb, a->q_ss, a->q_sh, a->qo_sb, a->qo_ss, a->qo_sh, a->q_heads};
-  P.k = Side{a->k, a->ko, a->k_sb, a->k_ss, a->k_sh, a->ko_sb, a->ko_ss, a->ko_sh, a->k_heads};
+  P.q = side(*a, a->q, a->qo, a->q_st, a->qo_st, a->q_heads);
+  P.k = side(*a, a->k, a->ko, a->k_st, a->ko_st, a->k_heads);
+  const int size = a->dtype == 2 ? 4 : 2, bytes = access_bytes(*a, P.q, P.k, size), v = bytes / size;
   P.positions = a->positions; P.pb = a->pos_sb; P.ps = a->pos_ss; P.pos64 = a->pos64;
   P.freqs = a->freqs; P.magnitude = a->magnitude; P.sign = a->backward ? -1.f : 1.f;
   P.tokens = tokens; P.S = a->S; P.hd = a->hd; P.rot = a->rot;

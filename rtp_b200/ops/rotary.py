@@ -6,6 +6,7 @@ model's own tables (``models.llama.rope_tables``, ``ops.kernels.rope``) stay for
 0, 1, 2, ..."""
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -16,20 +17,6 @@ LAYOUTS = ("half", "interleaved")
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
 
-class RotaryArgs(C.Structure):
-    _fields_ = [
-        ("q", C.c_void_p), ("k", C.c_void_p), ("qo", C.c_void_p), ("ko", C.c_void_p),
-        ("q_sb", C.c_longlong), ("q_ss", C.c_longlong), ("q_sh", C.c_longlong),
-        ("k_sb", C.c_longlong), ("k_ss", C.c_longlong), ("k_sh", C.c_longlong),
-        ("qo_sb", C.c_longlong), ("qo_ss", C.c_longlong), ("qo_sh", C.c_longlong),
-        ("ko_sb", C.c_longlong), ("ko_ss", C.c_longlong), ("ko_sh", C.c_longlong),
-        ("positions", C.c_void_p), ("pos_sb", C.c_longlong), ("pos_ss", C.c_longlong),
-        ("freqs", C.c_void_p), ("magnitude", C.c_float),
-        ("pos64", C.c_int), ("B", C.c_int), ("S", C.c_int), ("q_heads", C.c_int), ("k_heads", C.c_int), ("hd", C.c_int),
-        ("rot", C.c_int), ("half_layout", C.c_int), ("dtype", C.c_int), ("backward", C.c_int),
-    ]
-
-
 _declared = False
 
 
@@ -37,7 +24,7 @@ def _L():
     global _declared
     L = _lib.lib()
     if not _declared:
-        L.rtp_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
+        L.rtp_rotary.argtypes = [C.c_char_p, C.c_void_p]
         L.rtp_rotary_last_error.restype = C.c_char_p
         _declared = True
     return L
@@ -80,7 +67,24 @@ def rotary_magnitude(scaling="none", factor=1.0):
     return 0.1 * math.log(factor) + 1.0 if scaling == "yarn" and factor > 1 else 1.0
 
 
+def _good_args(q, k, positions, freqs, layout):
+    a, p, f = q.shape, positions.shape, freqs.shape
+    if len(a) != 4 or len(f) != 1 or not 0 < 2 * f[0] <= a[3] or layout not in LAYOUTS:
+        return False
+    if not (p == a[1:2] or p == a[:2] or (len(p) == 2 and p[0] == 1 and p[1] == a[1])):
+        return False
+    if k is not None:
+        b = k.shape
+        if len(b) != 4 or b[0] != a[0] or b[1] != a[1] or b[3] != a[3] or k.dtype != q.dtype or k.device != q.device:
+            return False
+    on = q.device
+    return q.dtype in _TYPES and positions.dtype in (torch.int64, torch.int32) and freqs.dtype == torch.float64 and positions.device == on and \
+        freqs.device == on
+
+
 def check_args(q, k, positions, freqs, layout):
+    if _good_args(q, k, positions, freqs, layout):
+        return
     if layout not in LAYOUTS:
         raise ValueError(f"unknown layout {layout!r}: one of {LAYOUTS}")
     if q.dim() != 4:
@@ -107,20 +111,9 @@ def kernel_takes(q):
     return q.is_cuda and q.dtype in _TYPES and q.shape[3] <= 256 and q.shape[3] % 2 == 0
 
 
-def _side(t, o):
-    """(tensor, its output, addresses, strides in and out, heads) of q or k; strides of a single batch entry, position or head do not
-    matter.  ``o``: where to (None: a new contiguous tensor)."""
-    if t is None:
-        return None, None, None, None, (0, 0, 0), (0, 0, 0), 0
-    if t.stride(3) != 1:
-        t = t.contiguous()
-    if o is None:
-        o = torch.empty_like(t, memory_format=torch.contiguous_format)
-    B, S, H, _ = t.shape
-    a, b = t.stride(), o.stride()
-    if B == 1 or S == 1 or H == 1:
-        a, b = ([s if n > 1 else 0 for s, n in zip(st, t.shape)] for st in (a, b))
-    return t, o, t.data_ptr(), o.data_ptr(), a[:3], b[:3], H
+# RtpRotary (csrc/kernels.h) as it lies in memory: packing the numbers takes a quarter of the time that filling a ctypes structure does
+_PACK = struct.Struct("@4P16qP2qPf10i0P").pack
+_NO_STRIDES = (0, 0, 0, 0)
 
 
 def _rotate(q, k, positions, freqs, half, magnitude, backward, qo=None, ko=None):
@@ -129,16 +122,33 @@ def _rotate(q, k, positions, freqs, half, magnitude, backward, qo=None, ko=None)
     if one.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(one.device):
             return _rotate(q, k, positions, freqs, half, magnitude, backward, qo, ko)
-    B, S, _, hd = one.shape
-    q, qo, qp, qop, qs, qos, H = _side(q, qo)         # copies live until the launch
-    k, ko, kp, kop, ks, kos, Hk = _side(k, ko)
+    qp = kp = qop = kop = H = Hk = 0
+    qs = ks = qos = kos = _NO_STRIDES
+    if q is not None:
+        qs = q.stride()
+        if qs[3] != 1:
+            q = q.contiguous()                        # lives until the launch, as k's below
+            qs = q.stride()
+        if qo is None:
+            qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        B, S, H, hd = q.shape
+        qp, qop, qos = q.data_ptr(), qo.data_ptr(), qo.stride()
+    if k is not None:
+        ks = k.stride()
+        if ks[3] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if ko is None:
+            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+        B, S, Hk, hd = k.shape
+        kp, kop, kos = k.data_ptr(), ko.data_ptr(), ko.stride()
     freqs = freqs.contiguous()
     st = positions.stride()
-    a = RotaryArgs(qp, kp, qop, kop, *qs, *ks, *qos, *kos, positions.data_ptr(), st[0] if len(st) == 2 and positions.shape[0] > 1 else 0,
-                   st[-1], freqs.data_ptr(), magnitude, positions.dtype == torch.int64, B, S, H, Hk, hd, 2 * freqs.shape[0], half,
-                   _TYPES[one.dtype], backward)
+    a = _PACK(qp, kp, qop, kop, *qs, *ks, *qos, *kos, positions.data_ptr(), st[0] if len(st) == 2 and positions.shape[0] > 1 else 0, st[-1],
+              freqs.data_ptr(), magnitude, positions.dtype == torch.int64, B, S, H, Hk, hd, 2 * freqs.shape[0], half, _TYPES[one.dtype],
+              backward)
     L = _L()
-    if L.rtp_rotary(C.byref(a), _lib.stream_ptr()) != 0:
+    if L.rtp_rotary(a, _lib.stream_ptr()) != 0:
         raise RuntimeError("rotary: " + L.rtp_rotary_last_error().decode())
     _lib.launches += 1
     return qo, ko
@@ -156,8 +166,9 @@ class _RotaryFn(torch.autograd.Function):
     def backward(ctx, dq, dk):
         positions, freqs = ctx.saved_tensors
         half, magnitude, backward = ctx.cfg
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
+        needs = ctx.needs_input_grad
+        dq = dq if needs[0] else None
+        dk = dk if needs[1] else None
         if dq is None and dk is None:
             return (None,) * 7
         # the transposed map is the same one with the angles negated

@@ -95,3 +95,19 @@ def test_frequency_refusals():
 def test_kernel_front_end_refuses_cpu_tensors():
     with pytest.raises(ValueError):
         R.rotary(**_args())
+
+
+def test_arguments_as_they_lie_in_memory():
+    """The kernels' argument structures, packed: their sizes, and each field of the windowed attention's."""
+    from rtp_b200.ops import _lib, flash
+    import ctypes as C
+    assert len(R._PACK(*range(21), *range(3), 1.0, *range(10))) == 4 * 8 + 16 * 8 + 8 + 16 + 8 + 4 + 10 * 4 + 4
+    refs = [[100 * r + i for i in range(8)] for r in range(8)]
+    a = _lib.WindowArgs.from_buffer_copy(flash._PACK(*sum(refs, []), 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 0.5, 0.25, 14, 15, 16, 17, 18, 19, 20, 21, 22))
+    f = a.f
+    for name, want in zip(("q", "k", "v", "o", "dout", "dq", "dk", "dv"), refs):
+        assert [getattr(getattr(f, name), n) or 0 for n, _ in _lib.FlashRef._fields_] == want
+    names = [n for n, _ in _lib.FlashArgs._fields_][8:]
+    assert [getattr(f, n) for n in names] == [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 0.5, 0.25, 14, 15, 16, 17]
+    assert (a.kv_heads, a.window, a.sinks, a.scratch, a.scratch_bytes) == (18, 19, 20, 21, 22)
+    assert C.sizeof(a) == 536
