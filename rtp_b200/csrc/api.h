@@ -29,17 +29,18 @@ typedef struct {
 int rtp_gemm(const RtpGemmArgs* args, void* stream);
 
 // Gated feed-forward block y = (silu(x Wg^T) * (x Wu^T)) Wd^T on this GPU alone: x [T, D], w_gu [2 F, D] (the rows of Wg before those of
-// Wu), w_d [O, F]; D, F and O multiples of 8, rows 16-byte aligned, everything bf16 with fp32 sums; gate, up, their product h and their
-// gradients are rounded to bf16.  gu, dgu [T, 2 F], h [T, F], y [T, O], dx [T, D], dw_gu and dw_d are dense.
+// Wu), w_d [O, F]; D, F and O multiples of 8, rows 16-byte aligned, everything bf16 with fp32 sums; gate and up are rounded to bf16 where
+// they are kept, their product h and their gradients for the products behind them.  gu, dgu [T, 2 F], h [T, F], y [T, O], dx [T, D], dw_gu and dw_d are dense.
 typedef struct {
   int T, D, F, O;
   const void* x; long long ldx;
   const void* w_gu; long long ld_gu;
   const void* w_d; long long ld_d;
   void* gu;                                   // the two projections, for the backward (null: not kept)
-  void* h;                                    // workspace
+  void* h;                                    // [T, F]: the product
   void* y;
-  int whole;                                  // 1: sums in the order of separate layers (products of few rows are not cut into slices)
+  // 1: the bits of separate layers (gate and up are rounded before their product, products of few rows are not cut into slices)
+  int whole;
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;   // rtp_gated_fwd_scratch() bytes, 16-byte aligned (none: null)
 } RtpGatedFwd;
@@ -53,7 +54,8 @@ typedef struct {
   const void* w_d; long long ld_d;
   const void* gu;                             // as the forward left it
   void* dgu;                                  // workspace
-  void* h;                                    // workspace, needed for dw_d
+  void* h;                                    // needed for dw_d: workspace, or
+  int h_kept;                                 // (1) the product as the forward left it
   void *dx, *dw_gu, *dw_d;                    // each may be null
   int whole;
   unsigned long long* status;

@@ -1644,7 +1644,7 @@ int rtp_gated_fwd(const RtpGatedFwd* a, void* stream) {
   up.a = a->x; up.lda = a->ldx; up.b = a->w_gu; up.ldb = a->ld_gu;
   up.M = a->T; up.N = 2 * a->F; up.K = a->D;
   up.d = a->h; up.ldd = a->F;
-  up.gate = 1; up.gu = a->gu; up.ldgu = 2ll * a->F;
+  up.gate = 1; up.gate_rounds = a->whole; up.gu = a->gu; up.ldgu = 2ll * a->F;
   SplitJobs down = gated_down(*a);
   return run_local(&up, 1, a->status, 0, stream) || run_split(down, a->scratch, a->scratch_bytes, a->status, stream) ? -1 : 0;
 }
@@ -1656,7 +1656,7 @@ int rtp_gated_bwd(const RtpGatedBwd* a, void* stream) {
   rtp::LocalGemm h = {};
   h.a = a->dy; h.lda = a->ldy; h.b = a->w_d; h.ldb = a->ld_d; h.b_mn = 1;
   h.M = a->T; h.N = a->F; h.K = a->O;
-  h.d = a->dw_d ? a->h : nullptr; h.ldd = a->F;
+  h.d = a->dw_d && !a->h_kept ? a->h : nullptr; h.ldd = a->F;
   h.gate = 2; h.gu = const_cast<void*>(a->gu); h.ldgu = 2ll * a->F; h.dgu = a->dgu; h.lddgu = 2ll * a->F;
   if (run_local(&h, 1, a->status, 0, stream)) return -1;
   SplitJobs grads = gated_grads(*a);

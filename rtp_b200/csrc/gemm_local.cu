@@ -74,7 +74,7 @@ struct alignas(64) Params {
   // gated feed-forward (see LocalGemm::gate); gate_cols: F
   __nv_bfloat16 *gu, *dgu;
   long long ldgu, lddgu;
-  int gate_cols;
+  int gate_cols, gate_rounds;
   Job job[MAXJ];
 };
 
@@ -142,8 +142,8 @@ __device__ __forceinline__ int tile_kblocks(const Job& J, int s, int row0) {
 // [2 F, K] weights of two halves that a GEMM of its own would write and a pass of its own read back.
 // GATE 2: the epilogue turns the gradient of the product into those of gate and up, which it reads, and makes the product again for the
 // weight gradient behind it.
-// Both round what they hand on to bf16 as the separate launches did (the stored gate and up are what the product is made of), so the
-// fused block gives their bits.
+// `gate_rounds`: the product is made of gate and up as they are stored, in bf16, as separate launches make it, whose bits this gives;
+// without it, of the sums in fp32: one rounding less in front of the down projection.
 template <bool PAIR, int MAXJ, bool SRC, bool FUN, bool FILL, int GATE>
 __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_constant__ Params<MAXJ> P) {
   extern __shared__ uint8_t smem_raw[];
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
         if (!good) { ok = false; break; }
         tc_fence_after();
         waited = true;
-        // 32 columns of both at a time: two staged rows of 64 bytes a thread, 16-byte chunk q at q ^ (row / 2) % 4
+        // 32 columns of both at a time, through staged rows of 64 bytes a thread, 16-byte chunk q at q ^ (row / 2) % 4
         const int cols = bn >> 1, per = cols >> 6;         // columns of a tile, pieces of a warp
         uint8_t* mine = stg + lane * 64;
         const int sw = (lane >> 1) & 3;
@@ -420,30 +420,39 @@ __global__ void __launch_bounds__(kThreads, 1) local_gemm_kernel(const __grid_co
           tmem_ld_32x32(acc_addr, ra[0]);
           tmem_ld_32x32(acc_addr + (uint32_t)cols, ra[1]);
           tmem_ld_wait();
+          uint32_t w[2][16], hw[16];
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int i = 0; i < 16; ++i) {
+            float g0 = __uint_as_float(ra[0][2 * i]), g1 = __uint_as_float(ra[0][2 * i + 1]);
+            float u0 = __uint_as_float(ra[1][2 * i]), u1 = __uint_as_float(ra[1][2 * i + 1]);
+            w[0][i] = pack_bf16(g0, g1);
+            w[1][i] = pack_bf16(u0, u1);
+            if (P.gate_rounds) { g0 = bf16_lo(w[0][i]); g1 = bf16_hi(w[0][i]); u0 = bf16_lo(w[1][i]); u1 = bf16_hi(w[1][i]); }
+            hw[i] = pack_bf16(swiglu(g0, u0), swiglu(g1, u1));
+          }
+          auto put = [&](uint8_t* to, const uint32_t* v) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = pack_bf16(__uint_as_float(ra[t][8 * q + 2 * i]), __uint_as_float(ra[t][8 * q + 2 * i + 1]));
-              *reinterpret_cast<uint4*>(mine + t * 2048 + ((q ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          __syncwarp();
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(to + ((q ^ sw) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          };
           const int col = tn * cols + pc * 32 + (lane & 3) * 8;
+          auto out = [&](const uint8_t* from, __nv_bfloat16* to, long long pitch) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = 8 * k + (lane >> 2), row = row0 + r;
-            const uint8_t* at = stg + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4);
-            const uint4 g = *reinterpret_cast<const uint4*>(at), u = *reinterpret_cast<const uint4*>(at + 2048);
-            if (row >= M || col >= P.gate_cols) continue;
-            if (P.gu) {
-              __nv_bfloat16* to = P.gu + (long long)row * P.ldgu + col;
-              *reinterpret_cast<uint4*>(to) = g;
-              *reinterpret_cast<uint4*>(to + P.gate_cols) = u;
+            for (int k = 0; k < 4; ++k) {
+              const int r = 8 * k + (lane >> 2), row = row0 + r;
+              if (row < M && col < P.gate_cols)
+                *reinterpret_cast<uint4*>(to + (long long)row * pitch + col) = *reinterpret_cast<const uint4*>(from + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
             }
-            auto two = [](uint32_t a, uint32_t b) { return pack_bf16(swiglu(bf16_lo(a), bf16_lo(b)), swiglu(bf16_hi(a), bf16_hi(b))); };
-            *reinterpret_cast<uint4*>(d + (long long)row * ldd + col) = make_uint4(two(g.x, u.x), two(g.y, u.y), two(g.z, u.z), two(g.w, u.w));
+          };
+          put(mine, hw);
+          if (P.gu) put(mine + 2048, w[0]);
+          __syncwarp();
+          out(stg, d, ldd);
+          if (P.gu) {
+            out(stg + 2048, P.gu, P.ldgu);
+            __syncwarp();
+            put(mine, w[1]);
+            __syncwarp();
+            out(stg, P.gu + P.gate_cols, P.ldgu);
           }
           __syncwarp();
         }
@@ -902,6 +911,7 @@ int run(const Item* it, int n, int pair_policy, unsigned long long* status, unsi
     J.N = x.N; J.tiles_n = (x.N + J.bn - 1) / J.bn;
     if (x.gate) {
       P.gate_cols = x.gate == 1 ? x.N / 2 : x.N;
+      P.gate_rounds = x.gate_rounds;
       P.gu = reinterpret_cast<__nv_bfloat16*>(x.gu); P.ldgu = x.ldgu;
       P.dgu = reinterpret_cast<__nv_bfloat16*>(x.dgu); P.lddgu = x.lddgu;
     }

@@ -294,8 +294,8 @@ def gated_mlp(x, w_gate_up, w_down):
     of ``Wu``), ``w_down`` [O, F] -> [..., O].
 
     bf16 CUDA tensors whose sizes are multiples of 8 run on the tcgen05 GEMM kernel with the activation and the product in its epilogue
-    (``ops/mlp.py``): sums in fp32; gate, up, their product and their gradients are rounded to bf16, as the operands of the
-    products behind them."""
+    (``ops/mlp.py``): sums in fp32; the product of gate and up and the gradients of both are rounded to bf16, as the operands
+    of the products behind them, and gate and up where they are kept for backward."""
     from . import mlp
     if get_backend() != "functional" and x.dim() and w_gate_up.dim() == 2 and w_down.dim() == 2 and mlp.kernel_takes(x, w_gate_up, w_down):
         return mlp.gated_mlp(x, w_gate_up, w_down)

@@ -25,7 +25,7 @@ class GatedBwd(C.Structure):
         ("T", C.c_int), ("D", C.c_int), ("F", C.c_int), ("O", C.c_int),
         ("x", C.c_void_p), ("ldx", C.c_longlong), ("dy", C.c_void_p), ("ldy", C.c_longlong),
         ("w_gu", C.c_void_p), ("ld_gu", C.c_longlong), ("w_d", C.c_void_p), ("ld_d", C.c_longlong),
-        ("gu", C.c_void_p), ("dgu", C.c_void_p), ("h", C.c_void_p), ("dx", C.c_void_p), ("dw_gu", C.c_void_p), ("dw_d", C.c_void_p),
+        ("gu", C.c_void_p), ("dgu", C.c_void_p), ("h", C.c_void_p), ("h_kept", C.c_int), ("dx", C.c_void_p), ("dw_gu", C.c_void_p), ("dw_d", C.c_void_p),
         ("whole", C.c_int), ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
     ]
 
@@ -86,7 +86,7 @@ def _check(rc, what, launches):
 
 
 def gated_fwd(x, w_gu, w_d, keep, whole=False):
-    """(y, gate | up or None) of [T, D] rows.  ``whole``: sums in the order of separate layers."""
+    """(y, gate | up or None, their product) of [T, D] rows.  ``whole``: the bits of separate layers."""
     if x.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(x.device):
             return gated_fwd(x, w_gu, w_d, keep, whole)
@@ -99,21 +99,24 @@ def gated_fwd(x, w_gu, w_d, keep, whole=False):
     L = _L()
     s = _scratch(L, "fwd", a, x.device)
     _check(L.rtp_gated_fwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_fwd", 2 if s is None else 3)
-    return y, gu
+    return y, gu, h
 
 
-def gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d, whole=False):
-    """Fills those of dx [T, D], dw_gu [2 * F, D] and dw_d [O, F] (dense) that are not None."""
+def gated_bwd(x, dy, w_gu, w_d, gu, h, dx, dw_gu, dw_d, whole=False):
+    """Fills those of dx [T, D], dw_gu [2 * F, D] and dw_d [O, F] (dense) that are not None.  ``h``: the product of gate and up as the
+    forward left it (None: made again for dw_d)."""
     if x.device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(x.device):
-            return gated_bwd(x, dy, w_gu, w_d, gu, dx, dw_gu, dw_d, whole)
+            return gated_bwd(x, dy, w_gu, w_d, gu, h, dx, dw_gu, dw_d, whole)
     T, D = x.shape
     O, F = w_d.shape
     dgu = torch.empty_like(gu)
-    h = x.new_empty(T, F) if dw_d is not None else None
-    p = [t.data_ptr() if t is not None else None for t in (h, dx, dw_gu, dw_d)]
+    kept = h is not None
+    if not kept and dw_d is not None:
+        h = x.new_empty(T, F)
+    ph, *p = [t.data_ptr() if t is not None else None for t in (h, dx, dw_gu, dw_d)]
     a = GatedBwd(T, D, F, O, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), w_gu.data_ptr(), w_gu.stride(0), w_d.data_ptr(),
-                 w_d.stride(0), gu.data_ptr(), dgu.data_ptr(), *p, whole, _lib.status_word(x.device).data_ptr(), None, 0)
+                 w_d.stride(0), gu.data_ptr(), dgu.data_ptr(), ph, kept, *p, whole, _lib.status_word(x.device).data_ptr(), None, 0)
     L = _L()
     s = _scratch(L, "bwd", a, x.device)
     _check(L.rtp_gated_bwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_bwd", 2 if s is None else 3)
@@ -127,12 +130,14 @@ class _GatedMlpFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gu, w_d, owners, rebuild, needs_bwd):
         x2, wg, wd = _rows(x.reshape(-1, x.shape[-1])), _rows(w_gu), _rows(w_d)
-        y, gu = gated_fwd(x2, wg, wd, needs_bwd, owners is not None)
+        y, gu, h = gated_fwd(x2, wg, wd, needs_bwd, owners is not None)
         if needs_bwd:
             kind, srcs = rebuild if rebuild is not None else (None, (x2,))
             ctx.kind, ctx.tensors = kind, [torch.is_tensor(s) for s in srcs]
             ctx.consts = [s for s in srcs if not torch.is_tensor(s)]
-            ctx.save_for_backward(gu, *(() if owners else (wg, wd)), *[s for s in srcs if torch.is_tensor(s)])
+            # h is kept for the down projection's gradient: made again of the rounded gate and up it would have another error than the
+            # forward's.  Layers of a model make it again, as they do one by one.
+            ctx.save_for_backward(gu, *(() if owners else (wg, wd, h if ctx.needs_input_grad[2] else None)), *[s for s in srcs if torch.is_tensor(s)])
             ctx.owners, ctx.shape = owners, x.shape
         return y.view(*x.shape[:-1], w_d.shape[0])
 
@@ -140,7 +145,7 @@ class _GatedMlpFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         gu, *kept = ctx.saved_tensors
-        wg, wd = [_rows(o.linear.weight) for o in ctx.owners] if ctx.owners else (kept.pop(0), kept.pop(0))
+        wg, wd, h = (*[_rows(o.linear.weight) for o in ctx.owners], None) if ctx.owners else [kept.pop(0) for _ in range(3)]
         if ctx.kind is None:
             x2 = kept[0]
         else:
@@ -154,7 +159,7 @@ class _GatedMlpFn(torch.autograd.Function):
         grads = [None if not n else w.new_empty(w.shape) if f is None else f[:w.numel()].view(w.shape)
                  for w, f, n in zip((wg, wd), flats, ctx.needs_input_grad[1:3])]
         dx = x2.new_empty(x2.shape) if ctx.needs_input_grad[0] else None
-        gated_bwd(x2, dy2, wg, wd, gu, dx, *grads, ctx.owners is not None)
+        gated_bwd(x2, dy2, wg, wd, gu, h, dx, *grads, ctx.owners is not None)
         for o, f in zip(ctx.owners or (), flats):
             if f is not None:
                 o._last_flat_grad = f

@@ -97,18 +97,15 @@ def test_small_and_saturated_gates(scale):
 
 @pytest.mark.parametrize("n", [1000, 704])
 def test_bits_of_the_separate_launches(n):
-    """The fused launches round where the separate ones do; a product in slices (dx at 2 x 1000 columns) adds up in another order."""
-    import ctypes as C
+    """`whole`: the fused launches round where the separate ones do and add up in their order."""
     from rtp_b200.ops.gemm import gemm
     x, wgu, wd, dy = tensors(300, 256, n, 264)
-    L = mlp._L()
-    sliced = L.rtp_gated_bwd_scratch(C.byref(mlp.GatedBwd(T=300, D=256, F=n, O=264, dx=1))) > 0
-    assert sliced == (n == 1000) and L.rtp_gated_fwd_scratch(C.byref(mlp.GatedFwd(T=300, D=256, F=n, O=264))) == 0
-    leaves = [t.requires_grad_() for t in (x, wgu, wd)]
-    y = FO.gated_mlp(*leaves)
-    gx, gg, gd = torch.autograd.grad(y, leaves, dy)
+    y, kept, _ = mlp.gated_fwd(x, wgu, wd, True, True)
+    gx, gg, gd = torch.empty_like(x), torch.empty_like(wgu), torch.empty_like(wd)
+    mlp.gated_bwd(x, dy, wgu, wd, kept, None, gx, gg, gd, True)
     with torch.no_grad():
         gu = gemm(x, wgu)
+        assert torch.equal(gu, kept)
     gu.requires_grad_()
     h = FO.swiglu_packed(gu)
     with torch.no_grad():
@@ -117,12 +114,26 @@ def test_bits_of_the_separate_launches(n):
         assert torch.equal(gemm(dy, h, a_mn=True, b_mn=True), gd)
     (dgu,) = torch.autograd.grad(h, gu, dh)
     with torch.no_grad():
-        if sliced:       # sums in fp32 either way, one rounding to bf16
-            a, b = gemm(dgu, wgu, b_mn=True).double(), gx.double()
-            assert bool(((a - b).abs() <= 2 * U * b.abs() + 2 * A * (dgu.double().abs() @ wgu.double().abs())).all())
-        else:
-            assert torch.equal(gemm(dgu, wgu, b_mn=True), gx)
+        assert torch.equal(gemm(dgu, wgu, b_mn=True), gx)
         assert torch.equal(gemm(dgu, x, a_mn=True, b_mn=True), gg)
+
+
+@pytest.mark.parametrize("T,D,n,O", [(8, 512, 2048, 512), (300, 256, 1000, 264), (9000, 128, 264, 128)])
+def test_the_product_is_rounded_once(T, D, n, O):
+    """y and the down projection's gradient have the error of a product rounded to bf16 once, not of rounded gates too."""
+    x, wgu, wd, dy = tensors(T, D, n, O, 5)
+    leaves = [t.detach().requires_grad_() for t in (x, wgu, wd)]
+    y = FO.gated_mlp(*leaves)
+    (gd,) = torch.autograd.grad(y, leaves[2], dy)
+    x, wgu, wd, dy = (t.double() for t in (x, wgu, wd, dy))
+    gu, egu = x @ wgu.t(), A * (x.abs() @ wgu.abs().t())
+    g, u, eg, eu = gu[:, :n], gu[:, n:], egu[:, :n], egu[:, n:]
+    h = g * torch.sigmoid(g) * u
+    eh = CROSS * (1.1 * eg * u.abs() + (g * torch.sigmoid(g)).abs() * eu + 1.1 * eg * eu) + (U + 1e-5) * h.abs()
+    for name, got, a, ea, b in (("y", y.detach(), h, eh, wd), ("dwd", gd, dy.t(), 0 * dy.t(), h.t())):
+        want = a @ b.t()
+        e = ea @ b.abs().t() + A * (a.abs() @ b.abs().t()) + (a.abs() @ eh if name == "dwd" else 0)
+        close(name, got, (want, e + U * want.abs()))
 
 
 def test_views():
