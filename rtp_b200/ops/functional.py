@@ -192,7 +192,8 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     (``j > p - window`` or ``j < sinks``).  ``sm_scale``: factor on the scores, ``hd ** -0.5`` by default.
 
     bf16 CUDA tensors of head_dim 64 or 128 run on the tcgen05 kernels (``csrc/flash_attn.cu``): scores in fp32, probabilities and their
-    gradients rounded to bf16 for the products, sums in fp32."""
+    gradients rounded to bf16 for the products, sums in fp32.  Hidden keys have a weight of exactly 0, which a dense product multiplies with
+    their rows too: values and, in backward, keys have to be finite there; keys that are not leave the output as it is."""
     if use_kernels(q) and q.dim() == 4 and q.shape[3] in (64, 128) and q.numel():
         from .flash import window_attention as run
         return run(q, k, v, window, sinks, sm_scale)

@@ -40,6 +40,8 @@ def gated_mlp(gate_up, down, x):
     if gate_up.linear.bias is not None or down.linear.bias is not None or gate_up.packed_parts != 2:
         return None
     from ..ops import mlp
+    if torch.nn.modules.module._has_any_global_hook():
+        return None
     if any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or m.inplace for m in (gate_up, down)):
         return None
     if not mlp.kernel_takes(x, wg, wd):

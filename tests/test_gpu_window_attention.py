@@ -236,3 +236,34 @@ def test_status_word_stays_clear():
     from rtp_b200.ops import _lib
     check(*tensors(1, 300, 300, 2, 2, 128), 100, 1)
     _lib.check_status("cuda:0")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), torch.finfo(torch.bfloat16).min])
+def test_hidden_keys_that_are_not_finite(bad, hd):
+    """They have no weight, whatever their scores: the output keeps its bits."""
+    for Sq, Sk, window, sinks in ((1, 300, 20, 2), (40, 300, 20, 2), (40, 300, 150, 0)):
+        q, k, v, _ = tensors(2, Sq, Sk, 4, 2, hd, Sk)
+        seen = ~hidden(Sq, Sk, window, sinks).all(0)
+        assert not bool(seen.all())
+        want = FO.window_attention(q, k, v, window, sinks=sinks)
+        k[:, ~seen] = bad
+        assert torch.equal(FO.window_attention(q, k, v, window, sinks=sinks), want)
+        assert bool(want.isfinite().all())
+
+
+def test_visible_values_that_are_not_finite_reach_the_output():
+    """A NaN in a query, a visible key or a visible value is one in the outputs and gradients that depend on it."""
+    for n in range(3):
+        q, k, v, do = tensors(1, 260, 260, 2, 1, 64, n)
+        (q, k, v)[n][0, 200, 0, 5] = float("nan")
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = FO.window_attention(*leaves, 50, sinks=1)
+        grads = torch.autograd.grad(o, leaves, do)
+        rows = o.isnan().any(-1)[0]                                       # [queries, heads]
+        if n == 0:
+            assert bool(rows[200, 0]) and int(rows.sum()) == 1
+        else:
+            assert bool(rows[200:250].all()) and not bool(rows[:128].any())
+        # dV = P^T dO does not depend on V
+        assert [bool(g.isnan().any()) for g in grads] == [True, True, n < 2]
