@@ -137,3 +137,16 @@ class ColumnParallelLinear(_RotatedLinearBase):
 class RowParallelLinear(_RotatedLinearBase):
     """Y = sum_j X[..., j] W_j^T + b with W sharded by input columns."""
     row = True
+
+
+_FORWARD = _RotatedLinearBase.forward
+
+
+def runs_plain_forward(module, kind) -> bool:
+    """Whether calling ``module`` is no more than the forward of ``kind`` (one of the two layers above) on the flat shard: no subclass,
+    wrapper, replaced or compiled forward, hook or in-place mode, and a weight that is the shard's memory.  Only then may a kernel of
+    several layers run in its place."""
+    return (type(module) is kind and kind.forward is _FORWARD and "forward" not in module.__dict__ and module._compiled_call_impl is None
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+            and not torch.nn.modules.module._has_any_global_hook() and not module.inplace
+            and module.linear.weight.data_ptr() == module._full_param.data_ptr())

@@ -29,20 +29,18 @@ def linear_ok(row, in_f, out_f, world):
 
 def gated_mlp(gate_up, down, x):
     """``down(silu(g) * u)`` of a packed column-parallel gate / up projection and a row-parallel down projection in the fused kernels of
-    one rank (``ops.mlp``); None: not a case for them (a ring of several ranks, biases, the in-place mode, hooks on the layers, a backward
-    pass that is not to make activations again)."""
-    from ..ops import functional as FO
+    one rank (``ops.mlp``); None: not a case for them (layers of another kind, with a forward or hooks of their own, a ring of several
+    ranks, biases, the in-place mode, a backward pass that is not to make activations again)."""
+    from ..module.linear import ColumnParallelLinear, RowParallelLinear, runs_plain_forward
+    from ..ops import functional as FO, mlp
     if torch.is_grad_enabled() and not FO.activation_recompute():
+        return None
+    if not runs_plain_forward(gate_up, ColumnParallelLinear) or not runs_plain_forward(down, RowParallelLinear):
         return None
     if gate_up.world_size != 1 or not use_fused(x, gate_up._full_param) or not use_fused(x, down._full_param):
         return None
     wg, wd = gate_up.linear.weight, down.linear.weight
     if gate_up.linear.bias is not None or down.linear.bias is not None or gate_up.packed_parts != 2:
-        return None
-    from ..ops import mlp
-    if torch.nn.modules.module._has_any_global_hook():
-        return None
-    if any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or m.inplace for m in (gate_up, down)):
         return None
     if not mlp.kernel_takes(x, wg, wd):
         return None
