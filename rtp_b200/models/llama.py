@@ -124,10 +124,10 @@ class LlamaBlock(nn.Module):
                                           magnitude=rotary_magnitude(cfg.rope_scaling, cfg.rope_factor),
                                           window=cfg.window or None, sinks=cfg.sinks)
 
-    def forward(self, x, *rope):
-        """``rope``: the cosine and sine tables, or positions and frequencies (see ``LlamaConfig.table_rope``)."""
+    def forward(self, x, cos, sin):
+        """``cos`` and ``sin``: the tables, or positions and frequencies in their place (see ``LlamaConfig.table_rope``)."""
         qkv = self.qkv(self.norm1(x))
-        x = x + self.proj((self._table_attention if self.cfg.table_rope else self._window_attention)(qkv, *rope))
+        x = x + self.proj((self._table_attention if self.cfg.table_rope else self._window_attention)(qkv, cos, sin))
         h = self.norm2(x)
         y = fused.gated_mlp(self.gate_up, self.down, h)
         return x + (self.down(FO.swiglu_packed(self.gate_up(h), self.N)) if y is None else y)
