@@ -8,6 +8,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "librtp_b200.so")
@@ -257,6 +258,16 @@ def check(rc: int, what: str):
             raise RotationTimeout(f"{what}: {e}") from None
         finally:
             _checking = False
+
+
+def through_autograd(*tensors) -> bool:
+    """Whether a call goes through its autograd function: a gradient is wanted, or a forward-mode derivative or a trace is being made,
+    which the function refuses and records.  Neither sees a launch: the one would come back as zero, the other without it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
 
 
 def stream_ptr() -> int:

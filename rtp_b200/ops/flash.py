@@ -348,7 +348,7 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     sm_scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
     if not 1e-30 < sm_scale < 1e30:
         raise ValueError(f"window attention: the kernels take a positive sm_scale, got {sm_scale}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.through_autograd(q, k, v):
         return _WindowFn.apply(q, k, v, window, sinks, sm_scale)
     return _window_fwd(q, k, v, window, sinks, sm_scale, False)[3]
 
@@ -386,5 +386,5 @@ class _RotaryWindowPackedFn(torch.autograd.Function):
 
 def rotary_window_attention_packed(qkv, positions, freqs, heads, kv_heads, layout, magnitude, window, sinks):
     """Kernel front-end of ``ops.functional.rotary_window_attention``."""
-    hd = qkv.shape[2] // (heads + 2 * kv_heads)
+    hd = int(qkv.shape[2]) // (heads + 2 * kv_heads)          # a tensor while a trace is made
     return _RotaryWindowPackedFn.apply(qkv, positions, freqs, layout == "half", float(magnitude), heads, kv_heads, hd, window, sinks)

@@ -36,7 +36,8 @@ def activation_recompute() -> bool:
 
 
 def _tag(out: torch.Tensor, kind: str, *srcs):
-    if _RECOMPUTE and torch.is_grad_enabled():
+    # a trace would keep the sources of the call that it was made from
+    if _RECOMPUTE and torch.is_grad_enabled() and torch._C._get_tracing_state() is None:
         out._rtp_recompute = (kind, srcs)
     return out
 
@@ -364,7 +365,7 @@ def rotary_window_attention(qkv, positions, freqs, heads, kv_heads=None, layout=
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
         raise ValueError(f"rotary_window_attention: qkv must be [B, S, (heads + 2 * kv_heads) * hd], got {tuple(qkv.shape)} for {heads} and {kv_heads} heads")
-    B, S, W = qkv.shape
+    B, S, W = map(int, qkv.shape)             # tensors while a trace is made
     hd = W // (heads + 2 * kv_heads)
     window = max(S, 1) if window is None else window
     q, k, v = qkv.view(B, S, heads + 2 * kv_heads, hd).split((heads, kv_heads, kv_heads), dim=2)

@@ -128,17 +128,16 @@ class _GatedMlpFn(torch.autograd.Function):
     input that can be made again (see ``ops.functional``), which is then not kept."""
 
     @staticmethod
-    def forward(ctx, x, w_gu, w_d, owners, rebuild, needs_bwd):
+    def forward(ctx, x, w_gu, w_d, owners, rebuild):
         x2, wg, wd = _rows(x.reshape(-1, x.shape[-1])), _rows(w_gu), _rows(w_d)
-        y, gu, h = gated_fwd(x2, wg, wd, needs_bwd, owners is not None)
-        if needs_bwd:
-            kind, srcs = rebuild if rebuild is not None else (None, (x2,))
-            ctx.kind, ctx.tensors = kind, [torch.is_tensor(s) for s in srcs]
-            ctx.consts = [s for s in srcs if not torch.is_tensor(s)]
-            # h is kept for the down projection's gradient: made again of the rounded gate and up it would have another error than the
-            # forward's.  Layers of a model make it again, as they do one by one.
-            ctx.save_for_backward(gu, *(() if owners else (wg, wd, h if ctx.needs_input_grad[2] else None)), *[s for s in srcs if torch.is_tensor(s)])
-            ctx.owners, ctx.shape = owners, x.shape
+        y, gu, h = gated_fwd(x2, wg, wd, True, owners is not None)
+        kind, srcs = rebuild if rebuild is not None else (None, (x2,))
+        ctx.kind, ctx.tensors = kind, [torch.is_tensor(s) for s in srcs]
+        ctx.consts = [s for s in srcs if not torch.is_tensor(s)]
+        # h is kept for the down projection's gradient: made again of the rounded gate and up it would have another error than the
+        # forward's.  Layers of a model make it again, as they do one by one.
+        ctx.save_for_backward(gu, *(() if owners else (wg, wd, h if ctx.needs_input_grad[2] else None)), *[s for s in srcs if torch.is_tensor(s)])
+        ctx.owners, ctx.shape = owners, x.shape
         return y.view(*x.shape[:-1], w_d.shape[0])
 
     @staticmethod
@@ -163,7 +162,7 @@ class _GatedMlpFn(torch.autograd.Function):
         for o, f in zip(ctx.owners or (), flats):
             if f is not None:
                 o._last_flat_grad = f
-        return (dx.view(ctx.shape) if dx is not None else None, *grads, None, None, None)
+        return (dx.view(ctx.shape) if dx is not None else None, *grads, None, None)
 
 
 def gated_mlp(x, w_gate_up, w_down, owners=None):
@@ -171,10 +170,8 @@ def gated_mlp(x, w_gate_up, w_down, owners=None):
     check_args(x, w_gate_up, w_down)
     if not kernel_takes(x, w_gate_up, w_down):
         raise ValueError(f"gated_mlp: the kernels take bf16 CUDA tensors with sizes that are multiples of 8, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    needs_bwd = torch.is_grad_enabled() and (x.requires_grad or w_gate_up.requires_grad or w_down.requires_grad)
-    # an input changed in place since its producer tagged it is kept
-    rebuild = getattr(x, "_rtp_recompute", None) if needs_bwd and x._version == 0 else None
-    if not needs_bwd:
+    if not _lib.through_autograd(x, w_gate_up, w_down):
         x2 = _rows(x.reshape(-1, x.shape[-1]))
         return gated_fwd(x2, _rows(w_gate_up), _rows(w_down), False, owners is not None)[0].view(*x.shape[:-1], w_down.shape[0])
-    return _GatedMlpFn.apply(x, w_gate_up, w_down, owners, rebuild, needs_bwd)
+    # an input changed in place since its producer tagged it is kept
+    return _GatedMlpFn.apply(x, w_gate_up, w_down, owners, getattr(x, "_rtp_recompute", None) if x._version == 0 else None)

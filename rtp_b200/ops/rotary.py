@@ -183,7 +183,7 @@ def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
     if not kernel_takes(q):
         raise ValueError(f"rotary: the kernel takes bf16, fp16 and fp32 CUDA tensors with an even head_dim up to 256, got {q.dtype} {tuple(q.shape)}")
     half, magnitude = layout == "half", float(magnitude)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _lib.through_autograd(q, k):
         return _RotaryFn.apply(q, k, positions, freqs, half, magnitude, False)
     return _rotate(q, k, positions, freqs, half, magnitude, False)
 
