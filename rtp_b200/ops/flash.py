@@ -345,6 +345,8 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     check_window_args(q, k, v, window, sinks)
     if not q.is_cuda or q.dtype != torch.bfloat16 or q.shape[3] not in (64, 128) or q.numel() == 0:
         raise ValueError(f"window attention: the kernels take bf16 CUDA tensors with head_dim 64 or 128, got {q.dtype} {tuple(q.shape)} on {q.device}")
+    if torch.is_grad_enabled() and torch.is_tensor(sm_scale) and sm_scale.requires_grad:
+        raise ValueError("window attention: the kernels have no gradient for sm_scale")
     sm_scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
     if not 1e-30 < sm_scale < 1e30:
         raise ValueError(f"window attention: the kernels take a positive sm_scale, got {sm_scale}")

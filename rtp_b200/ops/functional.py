@@ -35,6 +35,11 @@ def activation_recompute() -> bool:
     return _RECOMPUTE
 
 
+def _learned(*values) -> bool:
+    """Whether one of these constants of the kernels wants a gradient, which only the evaluation in PyTorch operations has."""
+    return torch.is_grad_enabled() and any(torch.is_tensor(v) and v.requires_grad for v in values)
+
+
 def _tag(out: torch.Tensor, kind: str, *srcs):
     # a trace would keep the sources of the call that it was made from
     if _RECOMPUTE and torch.is_grad_enabled() and torch._C._get_tracing_state() is None:
@@ -190,12 +195,13 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     are fine; ``H`` a multiple of ``Hk``, whose heads serve ``H / Hk`` neighbouring query heads each).
 
     The queries are the last ``Sq <= Sk`` positions: query i stands at ``p = i + Sk - Sq`` and sees key j if ``j <= p`` and
-    (``j > p - window`` or ``j < sinks``).  ``sm_scale``: factor on the scores, ``hd ** -0.5`` by default.
+    (``j > p - window`` or ``j < sinks``).  ``sm_scale``: factor on the scores, ``hd ** -0.5`` by default (one that
+    wants a gradient is evaluated in PyTorch operations).
 
     bf16 CUDA tensors of head_dim 64 or 128 run on the tcgen05 kernels (``csrc/flash_attn.cu``): scores in fp32, probabilities and their
     gradients rounded to bf16 for the products, sums in fp32.  Hidden keys have a weight of exactly 0, which a dense product multiplies with
     their rows too: values and, in backward, keys have to be finite there; keys that are not leave the output as it is."""
-    if use_kernels(q) and q.dim() == 4 and q.shape[3] in (64, 128) and q.numel():
+    if use_kernels(q) and q.dim() == 4 and q.shape[3] in (64, 128) and q.numel() and not _learned(sm_scale):
         from .flash import window_attention as run
         return run(q, k, v, window, sinks, sm_scale)
     from .flash import check_window_args
@@ -350,9 +356,10 @@ def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
 
     ``positions``: int64 / int32 [S] or [B, S], any values.  ``freqs``: float64 [rotary_dim / 2], see
     ``ops.rotary.rotary_frequencies``.  ``layout``: pairs ``(x[i], x[i + rotary_dim / 2])`` for ``"half"``, ``(x[2i], x[2i + 1])`` for
-    ``"interleaved"``.  ``magnitude``: factor on the rotated part (``ops.rotary.rotary_magnitude``)."""
+    ``"interleaved"``.  ``magnitude``: factor on the rotated part (``ops.rotary.rotary_magnitude``).  Frequencies or a
+    magnitude that want a gradient are evaluated in PyTorch operations."""
     from . import rotary as R
-    if R.kernel_takes(q) and get_backend() != "functional":
+    if R.kernel_takes(q) and get_backend() != "functional" and not _learned(freqs, magnitude):
         return R.rotary(q, k, positions, freqs, layout, magnitude)
     return R.rotary_plain(q, k, positions, freqs, layout, magnitude)
 
@@ -371,7 +378,7 @@ def rotary_window_attention(qkv, positions, freqs, heads, kv_heads=None, layout=
     q, k, v = qkv.view(B, S, heads + 2 * kv_heads, hd).split((heads, kv_heads, kv_heads), dim=2)
     R.check_args(q, k, positions, freqs, layout)
     flash.check_window_args(q, k, v, window, sinks)
-    if use_kernels(qkv) and hd in (64, 128) and qkv.numel() and qkv.is_contiguous() and qkv.data_ptr() % 16 == 0:
+    if use_kernels(qkv) and hd in (64, 128) and qkv.numel() and qkv.is_contiguous() and qkv.data_ptr() % 16 == 0 and not _learned(freqs, magnitude):
         return flash.rotary_window_attention_packed(qkv, positions, freqs, heads, kv_heads, layout, magnitude, window, sinks)
     q, k = rotary(q, k, positions, freqs, layout, magnitude)
     return window_attention(q, k, v, window, sinks).reshape(B, S, heads * hd)

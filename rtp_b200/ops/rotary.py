@@ -182,6 +182,8 @@ def rotary(q, k, positions, freqs, layout="half", magnitude=1.0):
     check_args(q, k, positions, freqs, layout)
     if not kernel_takes(q):
         raise ValueError(f"rotary: the kernel takes bf16, fp16 and fp32 CUDA tensors with an even head_dim up to 256, got {q.dtype} {tuple(q.shape)}")
+    if torch.is_grad_enabled() and (freqs.requires_grad or (torch.is_tensor(magnitude) and magnitude.requires_grad)):
+        raise ValueError("rotary: the kernel has no gradient for freqs and magnitude")
     half, magnitude = layout == "half", float(magnitude)
     if _lib.through_autograd(q, k):
         return _RotaryFn.apply(q, k, positions, freqs, half, magnitude, False)
