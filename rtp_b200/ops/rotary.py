@@ -108,7 +108,7 @@ def check_args(q, k, positions, freqs, layout):
 
 def kernel_takes(q):
     """CUDA tensors of one of the kernel's types and an even head_dim up to 256."""
-    return q.is_cuda and q.dtype in _TYPES and q.shape[3] <= 256 and q.shape[3] % 2 == 0
+    return q.is_cuda and q.dtype in _TYPES and q.dim() == 4 and q.shape[3] <= 256 and q.shape[3] % 2 == 0
 
 
 # RtpRotary (csrc/kernels.h) as it lies in memory: packing the numbers takes a quarter of the time that filling a ctypes structure does
