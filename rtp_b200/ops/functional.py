@@ -40,16 +40,25 @@ def _learned(*values) -> bool:
     return torch.is_grad_enabled() and any(torch.is_tensor(v) and v.requires_grad for v in values)
 
 
+def _versions(out, srcs):
+    return [t._version for t in (out, *srcs) if torch.is_tensor(t)]
+
+
 def _tag(out: torch.Tensor, kind: str, *srcs):
-    # a trace would keep the sources of the call that it was made from
-    if _RECOMPUTE and torch.is_grad_enabled() and torch._C._get_tracing_state() is None:
-        out._rtp_recompute = (kind, srcs)
+    # a trace would keep the sources of the call that it was made from; an inference tensor cannot be kept for a backward
+    if _RECOMPUTE and torch.is_grad_enabled() and torch._C._get_tracing_state() is None and \
+            not any(torch.is_tensor(t) and t.is_inference() for t in srcs):
+        out._rtp_recompute, out._rtp_versions = (kind, srcs), _versions(out, srcs)
     return out
 
 
 def recompute_tag(x: torch.Tensor):
-    """The (kind, sources) tag of a tensor produced by one of the ops below, or None."""
-    return getattr(x, "_rtp_recompute", None)
+    """The (kind, sources) tag of a tensor produced by one of the ops below, or None: also where the tensor or one of its sources has been
+    changed in place since (rebuilt from them it would be another one)."""
+    tag = getattr(x, "_rtp_recompute", None)
+    if tag is None or torch._C._get_tracing_state() is not None or x._rtp_versions != _versions(x, tag[1]):
+        return None
+    return tag
 
 
 def recompute(kind: str, srcs):

@@ -173,5 +173,5 @@ def gated_mlp(x, w_gate_up, w_down, owners=None):
     if not _lib.through_autograd(x, w_gate_up, w_down):
         x2 = _rows(x.reshape(-1, x.shape[-1]))
         return gated_fwd(x2, _rows(w_gate_up), _rows(w_down), False, owners is not None)[0].view(*x.shape[:-1], w_down.shape[0])
-    # an input changed in place since its producer tagged it is kept
-    return _GatedMlpFn.apply(x, w_gate_up, w_down, owners, getattr(x, "_rtp_recompute", None) if x._version == 0 else None)
+    from . import functional as FO
+    return _GatedMlpFn.apply(x, w_gate_up, w_down, owners, FO.recompute_tag(x))

@@ -18,6 +18,7 @@ import torch
 import torch.distributed as dist
 
 from ..ops import _lib, kernels as K
+from ..ops.functional import recompute_tag
 from .context import RingContext
 
 _engines: Dict[object, "FusedEngine"] = {}
@@ -462,7 +463,7 @@ def fused_linear(module, x, row=False):
     lin = module.linear
     spec = linear_spec(module, row, module.in_features, module.out_features, lin.weight, lin.bias)
     params = [p for p in (lin.weight, lin.bias) if p is not None]
-    spec.recompute = getattr(x, "_rtp_recompute", None)
+    spec.recompute = recompute_tag(x)
     return _FusedSubLinearFn.apply(spec, x, *params)
 
 
@@ -748,7 +749,7 @@ def fused_mha(owner, sub, x, *, is_causal=False, attn_mask=None, key_padding_mas
                             (o_ob - o_ow, sub.out_proj.bias.numel(), sub.out_proj.bias.shape)])
     if spec_out is None:
         return _mha_inplace(owner, sub, x, is_causal, attn_mask, key_padding_mask, training), None
-    spec_qkv.recompute = getattr(x, "_rtp_recompute", None)
+    spec_qkv.recompute = recompute_tag(x)
     qkv = _FusedSubLinearFn.apply(spec_qkv, x, sub.in_proj_weight, sub.in_proj_bias)       # [.., 3E] grouped per shard
     qkv2d = qkv.reshape(-1, 3 * E)
     causal = bool(is_causal) and attn_mask is None
