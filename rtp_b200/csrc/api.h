@@ -39,7 +39,8 @@ typedef struct {
   void* gu;                                   // the two projections, for the backward (null: not kept)
   void* h;                                    // [T, F]: the product
   void* y;
-  // 1: the bits of separate layers (gate and up are rounded before their product, products of few rows are not cut into slices)
+  // 1: the bits of separate layers (gate and up are rounded before their product, its gradient before theirs, products of few rows are
+  // not cut into slices)
   int whole;
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;   // rtp_gated_fwd_scratch() bytes, 16-byte aligned (none: null)

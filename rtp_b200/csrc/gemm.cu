@@ -1657,7 +1657,7 @@ int rtp_gated_bwd(const RtpGatedBwd* a, void* stream) {
   h.a = a->dy; h.lda = a->ldy; h.b = a->w_d; h.ldb = a->ld_d; h.b_mn = 1;
   h.M = a->T; h.N = a->F; h.K = a->O;
   h.d = a->dw_d && !a->h_kept ? a->h : nullptr; h.ldd = a->F;
-  h.gate = 2; h.gu = const_cast<void*>(a->gu); h.ldgu = 2ll * a->F; h.dgu = a->dgu; h.lddgu = 2ll * a->F;
+  h.gate = 2; h.gate_rounds = a->whole; h.gu = const_cast<void*>(a->gu); h.ldgu = 2ll * a->F; h.dgu = a->dgu; h.lddgu = 2ll * a->F;
   if (run_local(&h, 1, a->status, 0, stream)) return -1;
   SplitJobs grads = gated_grads(*a);
   return run_split(grads, a->scratch, a->scratch_bytes, a->status, stream);

@@ -40,7 +40,7 @@ struct LocalGemm {
   //    receives the two projections [M, 2 F].
   // 2: N = F, the product is the gradient of d: gu [M, 2 F] is read, dgu [M, 2 F] receives the gradients of the two projections and d
   //    (may be null) silu(gate) * up once more.
-  int gate, gate_rounds;           // gate_rounds: gate and up are rounded to bf16 before their product
+  int gate, gate_rounds;           // gate_rounds: gate, up and the gradient of their product are rounded to bf16 before they are used
   void* gu; long long ldgu;
   void* dgu; long long lddgu;
 };
