@@ -44,8 +44,9 @@ typedef struct {
   int whole;
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;   // rtp_gated_fwd_scratch() bytes, 16-byte aligned (none: null)
+  int launches;                               // out: two, and one for each product in slices
 } RtpGatedFwd;
-int rtp_gated_fwd(const RtpGatedFwd* args, void* stream);                 // two launches, and one for each product in slices
+int rtp_gated_fwd(RtpGatedFwd* args, void* stream);
 unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* args);
 typedef struct {
   int T, D, F, O;
@@ -61,8 +62,9 @@ typedef struct {
   int whole;
   unsigned long long* status;
   void* scratch; unsigned long long scratch_bytes;
+  int launches;                               // out: one, one for the gradients asked for, and one for each of those in slices
 } RtpGatedBwd;
-int rtp_gated_bwd(const RtpGatedBwd* args, void* stream);
+int rtp_gated_bwd(RtpGatedBwd* args, void* stream);
 unsigned long long rtp_gated_bwd_scratch(const RtpGatedBwd* args);
 
 // Batched GEMM over windows of two 2-D tensors: batch z = (zo, zi), zi = z % batch_inner.  Operand X (stored

@@ -1178,6 +1178,11 @@ struct SplitJobs {
     for (int i = 0; i < n; ++i) b += (unsigned long long)slices[i] * part_stride(job[i]) * 4;
     return b;
   }
+  int launches() const {
+    int k = n > 0;
+    for (int i = 0; i < n; ++i) k += slices[i] > 0;
+    return k;
+  }
 };
 int run_split(SplitJobs& s, void* scratch, unsigned long long bytes, unsigned long long* status, void* stream) {
   if (!s.n) return 0;
@@ -1637,7 +1642,7 @@ int rtp_gemm(const RtpGemmArgs* a, void* stream) {
   return launch<1>(params, grid, false, (cudaStream_t)stream, pair);
 }
 
-int rtp_gated_fwd(const RtpGatedFwd* a, void* stream) {
+int rtp_gated_fwd(RtpGatedFwd* a, void* stream) {
   if (gated_sizes(a->T, a->D, a->F, a->O)) return -1;
   if (!a->h || !a->y) return fail("gated feed-forward: outputs missing");
   rtp::LocalGemm up = {};
@@ -1646,11 +1651,12 @@ int rtp_gated_fwd(const RtpGatedFwd* a, void* stream) {
   up.d = a->h; up.ldd = a->F;
   up.gate = 1; up.gate_rounds = a->whole; up.gu = a->gu; up.ldgu = 2ll * a->F;
   SplitJobs down = gated_down(*a);
+  a->launches = 1 + down.launches();
   return run_local(&up, 1, a->status, 0, stream) || run_split(down, a->scratch, a->scratch_bytes, a->status, stream) ? -1 : 0;
 }
 unsigned long long rtp_gated_fwd_scratch(const RtpGatedFwd* a) { return a->T > 0 && a->F > 0 && a->O > 0 ? gated_down(*a).bytes() : 0; }
 
-int rtp_gated_bwd(const RtpGatedBwd* a, void* stream) {
+int rtp_gated_bwd(RtpGatedBwd* a, void* stream) {
   if (gated_sizes(a->T, a->D, a->F, a->O)) return -1;
   if (!a->gu || !a->dgu || (a->dw_d && !a->h)) return fail("gated feed-forward: workspace missing");
   rtp::LocalGemm h = {};
@@ -1660,6 +1666,7 @@ int rtp_gated_bwd(const RtpGatedBwd* a, void* stream) {
   h.gate = 2; h.gate_rounds = a->whole; h.gu = const_cast<void*>(a->gu); h.ldgu = 2ll * a->F; h.dgu = a->dgu; h.lddgu = 2ll * a->F;
   if (run_local(&h, 1, a->status, 0, stream)) return -1;
   SplitJobs grads = gated_grads(*a);
+  a->launches = 1 + grads.launches();
   return run_split(grads, a->scratch, a->scratch_bytes, a->status, stream);
 }
 unsigned long long rtp_gated_bwd_scratch(const RtpGatedBwd* a) {

@@ -17,6 +17,7 @@ class GatedFwd(C.Structure):
         ("x", C.c_void_p), ("ldx", C.c_longlong), ("w_gu", C.c_void_p), ("ld_gu", C.c_longlong),
         ("w_d", C.c_void_p), ("ld_d", C.c_longlong), ("gu", C.c_void_p), ("h", C.c_void_p), ("y", C.c_void_p), ("whole", C.c_int),
         ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
+        ("launches", C.c_int),
     ]
 
 
@@ -27,6 +28,7 @@ class GatedBwd(C.Structure):
         ("w_gu", C.c_void_p), ("ld_gu", C.c_longlong), ("w_d", C.c_void_p), ("ld_d", C.c_longlong),
         ("gu", C.c_void_p), ("dgu", C.c_void_p), ("h", C.c_void_p), ("h_kept", C.c_int), ("dx", C.c_void_p), ("dw_gu", C.c_void_p), ("dw_d", C.c_void_p),
         ("whole", C.c_int), ("status", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_ulonglong),
+        ("launches", C.c_int),
     ]
 
 
@@ -80,9 +82,9 @@ def _scratch(L, kind, a, device):
     return s
 
 
-def _check(rc, what, launches):
+def _check(rc, what, args):
     _lib.check(rc, what)
-    _lib.launches += launches - 1
+    _lib.launches += args.launches - 1
 
 
 def gated_fwd(x, w_gu, w_d, keep, whole=False):
@@ -97,8 +99,8 @@ def gated_fwd(x, w_gu, w_d, keep, whole=False):
     a = GatedFwd(T, D, F, O, x.data_ptr(), x.stride(0), w_gu.data_ptr(), w_gu.stride(0), w_d.data_ptr(), w_d.stride(0),
                  gu.data_ptr() if keep else None, h.data_ptr(), y.data_ptr(), whole, _lib.status_word(x.device).data_ptr(), None, 0)
     L = _L()
-    s = _scratch(L, "fwd", a, x.device)
-    _check(L.rtp_gated_fwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_fwd", 2 if s is None else 3)
+    scratch = _scratch(L, "fwd", a, x.device)           # noqa: F841 (lives until the launch)
+    _check(L.rtp_gated_fwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_fwd", a)
     return y, gu, h
 
 
@@ -118,8 +120,8 @@ def gated_bwd(x, dy, w_gu, w_d, gu, h, dx, dw_gu, dw_d, whole=False):
     a = GatedBwd(T, D, F, O, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0), w_gu.data_ptr(), w_gu.stride(0), w_d.data_ptr(),
                  w_d.stride(0), gu.data_ptr(), dgu.data_ptr(), ph, kept, *p, whole, _lib.status_word(x.device).data_ptr(), None, 0)
     L = _L()
-    s = _scratch(L, "bwd", a, x.device)
-    _check(L.rtp_gated_bwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_bwd", 2 if s is None else 3)
+    scratch = _scratch(L, "bwd", a, x.device)           # noqa: F841 (lives until the launch)
+    _check(L.rtp_gated_bwd(C.byref(a), _lib.stream_ptr()), "rtp_gated_bwd", a)
 
 
 class _GatedMlpFn(torch.autograd.Function):
