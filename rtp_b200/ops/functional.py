@@ -208,8 +208,10 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None):
     wants a gradient is evaluated in PyTorch operations).
 
     bf16 CUDA tensors of head_dim 64 or 128 run on the tcgen05 kernels (``csrc/flash_attn.cu``): scores in fp32, probabilities and their
-    gradients rounded to bf16 for the products, sums in fp32.  Hidden keys have a weight of exactly 0, which a dense product multiplies with
-    their rows too: values and, in backward, keys have to be finite there; keys that are not leave the output as it is."""
+    gradients rounded to bf16 for the products, sums in fp32.  They take the maximum before the scale, so ``sm_scale`` has to lie between
+    1e-30 and 1e30 there (``ValueError`` otherwise).  Hidden keys have a weight of exactly 0, which a dense product multiplies with
+    their rows too: values and, in backward, keys have to be finite there; keys that are not leave the output as it is.  Other tensors are
+    evaluated in PyTorch operations, with any scale and with all [B, H, Sq, Sk] scores in memory."""
     if use_kernels(q) and q.dim() == 4 and q.shape[3] in (64, 128) and q.numel() and not _learned(sm_scale):
         from .flash import window_attention as run
         return run(q, k, v, window, sinks, sm_scale)
