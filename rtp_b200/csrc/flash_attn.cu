@@ -242,9 +242,10 @@ __device__ __forceinline__ uint32_t keep_bits(const MaskArgs& m, unsigned long l
 }
 
 // Common set-up: barriers, TMEM, abort flag.  Returns the TMEM base.
-__device__ __forceinline__ uint32_t setup_cta(Ctl* ctl, const int* counts, int nbar, int warp, int lane) {
+template <typename Count>
+__device__ __forceinline__ uint32_t setup_cta(Ctl* ctl, Count count, int nbar, int warp, int lane) {
   if (warp == kProducerWarp) {
-    if (lane < nbar) mbar_init(&ctl->bar[lane], counts[lane]);
+    if (lane < nbar) mbar_init(&ctl->bar[lane], count(lane));
     if (lane == 31) ctl->abort_flag = 0;
     mbar_fence_init();
     __syncwarp();
@@ -548,12 +549,12 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
 
   // counts by barrier index: copies and commits 1 each, P (its first three quarters, its last) 4: one per row warp of the tile,
   // next work 1 and 10 (producer, issuer, eight row warps)
-  const int counts[23] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 10, 1};
+  auto count = [](int i) { return i == F_TAKEN ? 10 : i >= F_PFULL && i < F_OFULL ? 4 : 1; };
   // The first work is looked up before the wait for the previous kernel: its divisions took 1 000 clocks between set-up and the first
   // copy, of the 12 000 of a launch of one key block (4 x 8 heads of 64 x 64).
   const FwdWork first = fwd_work<WIN>(p, (int)blockIdx.x);
   asm volatile("" ::"r"(first.b), "r"(first.h), "r"(first.g0), "r"(first.nload));
-  const uint32_t tmem = setup_cta(ctl, counts, 23, warp, lane);
+  const uint32_t tmem = setup_cta(ctl, count, 23, warp, lane);
   volatile uint32_t* abort_flag = &ctl->abort_flag;
   unsigned long long* status = p.status;
   const unsigned long long tmo = p.timeout_ns;
@@ -888,23 +889,17 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
 // =====================================================================================================  backward
 // delta[b, h, q] = rowsum(dO * O), HD / 8 lanes a row.  Reads both once (8192 tokens x 16 heads of 128: 67 MB), apart from the
 // launch below so that its two kinds of CTAs need nothing of each other.
-template <int HD>
+// I: type of a row's number.  In 64 bits 524 288 rows of 128 take 58 us, in 32 bits 54; both behind a branch cost 0.5 us of the 14.6 of a
+// forward and backward of 8 x 8 heads of 128 x 128.
+template <int HD, typename I>
 __global__ void __launch_bounds__(256) flash_delta_kernel(DRef o, DRef g, float* __restrict__ delta, int Sq, int H, long long rows) {
   pdl_prologue();
   constexpr int LPR = HD / 8;
   const long long r = (blockIdx.x * 256ll + threadIdx.x) / LPR;
   const int c = threadIdx.x % LPR;
   float s = 0.f;
-  int h, b, q;                                               // rows in memory order: (batch, position, head)
-  if (rows <= 0x7fffffffll) {                                // in 64 bits 524 288 rows of 128 took 58 us, not 54
-    const uint32_t bs = (uint32_t)r / (uint32_t)H;
-    h = (int)((uint32_t)r - bs * (uint32_t)H);
-    b = (int)(bs / (uint32_t)Sq);
-    q = (int)(bs - (uint32_t)b * (uint32_t)Sq);
-  } else {
-    const long long bs = r / H;
-    h = (int)(r % H); b = (int)(bs / Sq); q = (int)(bs % Sq);
-  }
+  const I bs = (I)r / (I)H;                                  // rows in memory order: (batch, position, head)
+  const int h = (int)((I)r - bs * (I)H), b = (int)(bs / (I)Sq), q = (int)(bs - (I)b * (I)Sq);
   if (r < rows) {
     const uint4 x = __ldg(reinterpret_cast<const uint4*>(row_ptr(o, b, q, h)) + c);
     const uint4 y = __ldg(reinterpret_cast<const uint4*>(row_ptr(g, b, q, h)) + c);
@@ -1037,10 +1032,13 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
   const int nqb = (M.Sq + kBlk - 1) / kBlk, nkb = (M.Sk + kBlk - 1) / kBlk;
   // counts by barrier index: copies and commits 1; statistics 32 (lanes); P and dS, accumulators read 8 (one per row warp); next work
   // 1 and 10 (producer, issuer, eight row warps)
-  const int counts[28] = {1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 32, 32, 1, 1, 8, 1, 8, 1, 8, 1, 10, 1, 8, 8};
+  auto count = [](int i) {
+    return i == B_STAT || i == B_STAT + 1 ? 32 : i == B_TAKEN ? 10
+         : i == B_PFULL || i == B_DSFULL || i == B_ACCREAD || i == B_PTAIL || i == B_DSTAIL ? 8 : 1;
+  };
   const BwdWork first = bwd_work<WIN>(p, (int)blockIdx.x);       // before the wait for the previous kernel, as in forward
   asm volatile("" ::"r"(first.b), "r"(first.h), "r"(first.kb), "r"(first.qb));
-  const uint32_t tmem = setup_cta(ctl, counts, 28, warp, lane);
+  const uint32_t tmem = setup_cta(ctl, count, WIN ? 28 : 26, warp, lane);
   volatile uint32_t* abort_flag = &ctl->abort_flag;
   unsigned long long* status = p.status;
   const unsigned long long tmo = p.timeout_ns;
@@ -1409,11 +1407,13 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
           publish_rows(&bar[WIN ? B_DSTAIL : B_DSFULL], lane);
         }
       }
-      const int r0 = (w.kb >= 0 ? w.kb : w.qb) * kBlk + (warp & 3) * 32;      // the warp's first row
+      auto first_row = [&] { return (w.kb >= 0 ? w.kb : w.qb) * kBlk + (warp & 3) * 32; };      // of the warp
       // window: where the results go, looked up under the last product
+      [[maybe_unused]] int r0 = 0;
       [[maybe_unused]] __nv_bfloat16 *dst0 = nullptr, *dst1 = nullptr;
       [[maybe_unused]] long long pitch0 = 0, pitch1 = 0;
       if constexpr (WIN) {
+        r0 = first_row();
         if (w.kb < 0) {
           dst0 = row_ptr(p.dq, b, r0, h) + wg * (HD / 2);
           pitch0 = p.dq.ss;
@@ -1428,6 +1428,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_bwd_kernel(const __grid_con
       if (ok) ok = wait(B_ACC, n & 1u);
       if (!ok) break;
       tc_fence_after();
+      if constexpr (!WIN) r0 = first_row();
       const int nacc = ONE ? 3 : w.kb >= 0 ? 2 : 1;
       if constexpr (WIN) {
         // 32 columns at a time, one after the other: with all of them read at once, unrolled, the steps before spilled and their code had
@@ -1703,6 +1704,14 @@ int sink_pieces(const RtpWindowArgs* w, int sms) {
   return (int)std::max(1ll, std::min({all / other, room, all}));
 }
 int mask_kind(const RtpFlashArgs* a) { return a->mask ? 2 : a->kpm ? 1 : 0; }
+int launch_delta(const RtpFlashArgs* a, const FlashParams& P, cudaStream_t s) {
+  const long long rows = (long long)a->B * a->Sq * a->H, per = 256 / (a->head_dim / 8);
+  const bool small = rows <= 0x7fffffffll;
+  const cudaError_t e = launch_k(a->head_dim == 64 ? (small ? flash_delta_kernel<64, uint32_t> : flash_delta_kernel<64, unsigned long long>)
+                                                   : (small ? flash_delta_kernel<128, uint32_t> : flash_delta_kernel<128, unsigned long long>),
+                                 dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
+  return e == cudaSuccess ? 0 : ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
+}
 int launched(int e, const char* what) { return e == (int)cudaSuccess ? 0 : ffail(std::string(what) + ": " + cudaGetErrorString((cudaError_t)e)); }
 
 }  // namespace
@@ -1745,10 +1754,7 @@ int rtp_flash_bwd(const RtpFlashArgs* a, void* stream) {
   const int kind = one ? 2 : grid > 2 * device_sms();   // one or two rounds are over sooner without (16 heads of 1024 x 1024: 55 us, 60)
   cudaStream_t s = (cudaStream_t)stream;
   P.group = one ? BH : head_group(4ll * (a->Sq + a->Sk) * a->head_dim, BH);
-  const long long rows = (long long)a->B * a->Sq * a->H, per = 256 / (a->head_dim / 8);
-  const cudaError_t e = launch_k(a->head_dim == 64 ? flash_delta_kernel<64> : flash_delta_kernel<128>,
-                                 dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
-  if (e != cudaSuccess) return ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
+  if (launch_delta(a, P, s)) return -1;
   return launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, mask_kind(a), P.m.thresh != 0, kind, grid, stream),
                   "flash_bwd");
 }
@@ -1804,16 +1810,13 @@ int rtp_window_bwd(const RtpWindowArgs* w, void* stream) {
   P.by_group = divider(P.group);
   P.by_last_group = divider(BK % P.group ? BK % P.group : P.group);
   cudaStream_t s = (cudaStream_t)stream;
-  const long long rows = (long long)a->B * a->Sq * a->H, lanes = 256 / (a->head_dim / 8);
-  cudaError_t e = launch_k(a->head_dim == 64 ? flash_delta_kernel<64> : flash_delta_kernel<128>,
-                           dim3((unsigned)((rows + lanes - 1) / lanes)), dim3(256), 0, s, P.o, P.dout, P.delta, a->Sq, a->H, rows);
-  if (e != cudaSuccess) return ffail(std::string("flash_delta: ") + cudaGetErrorString(e));
+  if (launch_delta(a, P, s)) return -1;
   if (launched((a->head_dim == 64 ? rtp_flash_part_bwd64 : rtp_flash_part_bwd128)(&P, 3, 0, grid > 2 * device_sms(), grid, stream),
                "window_bwd"))
     return -1;
   if (!P.part) return 0;
   const long long items = (long long)BK * P.sink_blocks * 2 * (a->head_dim / 4) * kBlk;
-  e = launch_k(a->head_dim == 64 ? flash_sinks_kernel<64> : flash_sinks_kernel<128>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0,
+  const cudaError_t e = launch_k(a->head_dim == 64 ? flash_sinks_kernel<64> : flash_sinks_kernel<128>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0,
                s, (const float*)P.part, P.dk, P.dv, a->Sk, w->kv_heads, P.sink_blocks, P.pieces, items);
   return e == cudaSuccess ? 0 : ffail(std::string("flash_sinks: ") + cudaGetErrorString(e));
 }
