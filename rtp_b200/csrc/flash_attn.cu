@@ -858,7 +858,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       m_used = m_all;
     }
     if (ok && stores) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      // a row whose keys are all masked has no weights and gives 0; a window leaves every row a key, so its sum is 0 only where all scores
+      // that a row sees are -inf, and the quotient is undefined
+      const float inv = WIN || l > 0.f ? 1.f / l : 0.f;
       const float* xi = reinterpret_cast<const float*>(sK) + (t ^ 1) * (HD / 2) * 128;
       const int c0 = split ? t * OC : 0, c1 = split ? c0 + OC : 2 * OC;
       const uint32_t aR = lone ? lane_addr + 256u : aO;
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_fwd_kernel(const __grid_con
       }
       if (row < M.Sq && p.lse && !(split && t)) {
         const float mref = (m_used == -INFINITY) ? 0.f : m_used;
-        p.lse[(long long)bh * M.Sq + row] = l > 0.f ? mref + log2f(l) : INFINITY;
+        p.lse[(long long)bh * M.Sq + row] = WIN || l > 0.f ? mref + log2f(l) : INFINITY;
       }
       tc_fence_before();               // O has been read before the next P is announced
     }
