@@ -4,6 +4,7 @@
 below has a plain PyTorch evaluation for CPU / fp32 tensors so that the same model code runs on gloo."""
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from ..parallel.context import get_backend
 
@@ -36,8 +37,15 @@ def activation_recompute() -> bool:
 
 
 def _learned(*values) -> bool:
-    """Whether one of these constants of the kernels wants a gradient, which only the evaluation in PyTorch operations has."""
-    return torch.is_grad_enabled() and any(torch.is_tensor(v) and v.requires_grad for v in values)
+    """Whether one of these constants of the kernels wants a gradient or carries a forward-mode derivative: only the evaluation in PyTorch
+    operations has them."""
+    for v in values:
+        if torch.is_tensor(v):
+            if v.requires_grad and torch.is_grad_enabled():
+                return True
+            if forward_ad._current_level >= 0 and forward_ad.unpack_dual(v).tangent is not None:
+                return True
+    return False
 
 
 def _versions(out, srcs):

@@ -4,6 +4,7 @@ Against central differences of the 64-bit evaluation: the inputs are fp32 or bf1
 the magnitudes of the summed terms is far below 1e-3 (bf16 results enter no gradient here but through the incoming one, which is 1)."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from rtp_b200.ops import flash, functional as FO, rotary as R
 
@@ -75,3 +76,21 @@ def test_the_kernels_refuse_them():
             R.rotary(q, None, pos, **kw)
     with pytest.raises(ValueError):
         flash.window_attention(q, q, q, 3, sm_scale=one)
+
+
+def test_forward_mode():
+    """A derivative along a constant, beside its gradient summed over the same output."""
+    q = torch.randn(1, 5, 2, 64, device="cuda").bfloat16()
+    f, pos = R.rotary_frequencies(64, theta=10.0, device="cuda"), torch.arange(5, device="cuda")
+    calls = [(lambda c: FO.rotary(q.float(), None, pos, f, magnitude=c)[0], torch.tensor(1.25, device="cuda")),
+             (lambda c: FO.rotary(q.float(), None, pos, c)[0], f),
+             (lambda c: FO.window_attention(q, q, q, 3, sm_scale=c), torch.tensor(0.2, device="cuda"))]
+    for call, at in calls:
+        along = torch.ones_like(at)
+        with fw.dual_level():
+            tangent = fw.unpack_dual(call(fw.make_dual(at, along))).tangent
+        assert tangent is not None
+        leaf = at.clone().requires_grad_()
+        (g,) = torch.autograd.grad(call(leaf).float().sum(), leaf)
+        # bf16 outputs have a tangent rounded to bf16 each: half a step of the 640 of them
+        assert abs(float(tangent.float().sum() - g.sum())) <= 2.0 ** -8 * float(tangent.float().abs().sum()) + 1e-4
