@@ -268,6 +268,8 @@ def _ref(t):
     """The fields of the FlashRef of a [B, S, H, hd] view with unit stride on hd."""
     sb, ss, sh, _ = t.stride()
     _, _, H, hd = t.shape
+    if H == 1:
+        sh = 0                     # any number, also one of more than 32 bits
     return t.data_ptr(), sb, ss, (H - 1) * sh + hd, 0, H, 0, sh
 
 
