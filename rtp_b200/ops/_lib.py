@@ -247,11 +247,7 @@ def check(rc: int, what: str):
         torch.cuda.synchronize()
         _checking = True
         try:
-            for w in list(_status_words.values()):
-                v = int(w.item())
-                if v:
-                    w.zero_()
-                    raise RotationTimeout(status_text(v))
+            check_status_words()
             for hook in _after_launch_hooks:
                 hook()
         except RotationTimeout as e:
@@ -306,10 +302,19 @@ class RotationTimeout(RuntimeError):
     """A bounded device-side wait expired; the kernel returned early and its outputs are invalid."""
 
 
-def check_status(device=None):
-    """Synchronously read the status word and raise RotationTimeout if a kernel reported an error."""
-    w = status_word(device)
+def _raise_if_set(w):
     v = int(w.item())
     if v != 0:
         w.zero_()
         raise RotationTimeout(status_text(v))
+
+
+def check_status(device=None):
+    """Synchronously read the status word and raise RotationTimeout if a kernel reported an error."""
+    _raise_if_set(status_word(device))
+
+
+def check_status_words():
+    """The same for the words of all devices that have one."""
+    for w in list(_status_words.values()):
+        _raise_if_set(w)

@@ -215,8 +215,10 @@ def workspace_bytes() -> int:
 
 
 def check_all():
+    """Raises for a bounded wait that expired in a kernel of any ring or outside one (flash attention, a model's gated block)."""
     for e in _engines.values():
         e.check()
+    _lib.check_status_words()
 
 
 # --------------------------------------------------------------------------------------------------
