@@ -162,8 +162,7 @@ class _GatedMlpFn(torch.autograd.Function):
         dx = x2.new_empty(x2.shape) if ctx.needs_input_grad[0] else None
         gated_bwd(x2, dy2, wg, wd, gu, h, dx, *grads, ctx.owners is not None)
         for o, f in zip(ctx.owners or (), flats):
-            if f is not None:
-                o._last_flat_grad = f
+            o._last_flat_grad = f                         # None: no gradient was asked for, and an earlier one is not this pass's
         return (dx.view(ctx.shape) if dx is not None else None, *grads, None, None)
 
 
